@@ -34,7 +34,7 @@ extern "C" {
 
 /* Bumped on every struct or semantic change; the binding refuses a library
  * reporting another value. */
-#define SDFR_ABI_VERSION 14
+#define SDFR_ABI_VERSION 15
 
 /* Element types of caller arrays. */
 enum {
@@ -355,6 +355,165 @@ SDFR_API int32_t sdfr_goal_yaw(const void* grid, int32_t grid_dtype, float quant
                                double reach_max, const void* pos, int32_t pos_dtype,
                                int64_t pos_stride, int64_t n, float* out, void* stream);
 SDFR_API const char* sdfr_goal_last_error(void);
+
+/* ---- A recurrent policy's operators ---------------------------------------
+ * What a policy that sees the renders needs beside them, and the reference
+ * has no counterpart of (its trainer stacks frames instead of keeping a
+ * memory, and draws and clips with torch): a short causal convolution and a
+ * selective state space scan over the decisions of a rollout or the tokens of
+ * a prompt, each with its gradients and, as the call of length 1, its step for
+ * one token; the draw of an action or token; the clipping of gradients.
+ *
+ * Element types are SDFR_F32, SDFR_F16 or SDFR_BF16, the same for all of a
+ * call's activations; parameters, states of the scan and their gradients are
+ * fp32. Channels (states of B and C, a row's logits) have unit stride; batch
+ * and step strides are in elements and may be anything that the caller's
+ * memory holds. `resets` (batch, length) bytes: nonzero where a sequence
+ * begins, whose step sees nothing of what came before; NULL = none. Sums go in
+ * a fixed order: the same call gives the same bits. All calls are asynchronous
+ * on `stream`, allocate nothing and may be captured; 0 or < 0
+ * (sdfr_recurrent_last_error()): -1 null pointer, -2 bad size or workspace,
+ * -3 bad type, -4 launch failure. */
+
+/* pre[t] = bias + sum_j weight[d, width-1-j] x[t-j], j < width; y = pre
+ * sigmoid(pre) with silu, else pre. */
+typedef struct SdfrConv {
+    const void* x;           /* (batch, length, channels) */
+    int64_t x_b, x_t;
+    const float* weight;     /* (channels, width) dense, the last column weighs the present */
+    const float* bias;       /* (channels) or NULL */
+    const uint8_t* resets;
+    int64_t resets_b, resets_t;
+    const void* state;       /* (batch, width-1, channels) dense: the last inputs of the call before,
+                                oldest first; NULL = zeros */
+    void* y;                 /* (batch, length, channels) */
+    int64_t y_b, y_t;
+    void* state_out;         /* like state, cleared before the last reset; may be `state` itself in
+                                calls of up to 16 steps; NULL = not wanted */
+    int64_t length;
+    int32_t batch, channels;
+    int32_t width;           /* 1 to 8 */
+    int32_t dtype, silu;
+} SdfrConv;
+
+typedef struct SdfrConvGrad {
+    const void* dy;          /* gradient of y */
+    int64_t dy_b, dy_t;
+    const void* dstate_out;  /* gradient of state_out, dense, or NULL */
+    void* dx;                /* (batch, length, channels) dense */
+    void* dstate;            /* like state, or NULL */
+    float* dweight;          /* (channels, width) */
+    float* dbias;            /* (channels) or NULL */
+} SdfrConvGrad;
+
+SDFR_API int32_t sdfr_conv(const SdfrConv* conv, void* stream);
+/* The gradients of a call of sdfr_conv (its y and state_out are not read).
+ * `workspace`: sdfr_conv_grad_workspace_bytes() bytes, 64-byte aligned. */
+SDFR_API int64_t sdfr_conv_grad_workspace_bytes(const SdfrConv* conv);
+SDFR_API int32_t sdfr_conv_grad(const SdfrConv* conv, const SdfrConvGrad* grad, void* workspace,
+                                int64_t workspace_size, void* stream);
+
+/* With D = softplus(dt + dt_bias) (or dt + dt_bias), per channel d and state n:
+ * h[t] = exp(D A[d,n]) h[t-1] + D x[t] B[t,n]; y[t] = sum_n C[t,n] h[t] +
+ * skip[d] x[t], times z sigmoid(z) if there is a z. */
+typedef struct SdfrScan {
+    const void* x;           /* (batch, length, channels), as dt and z */
+    int64_t x_b, x_t;
+    const void* dt;
+    int64_t dt_b, dt_t;
+    const void* z;           /* or NULL */
+    int64_t z_b, z_t;
+    const void* B;           /* (batch, length, states) */
+    int64_t B_b, B_t;
+    const void* C;
+    int64_t C_b, C_t;
+    const float* A;          /* (channels, states) dense */
+    const float* skip;       /* (channels) or NULL */
+    const float* dt_bias;    /* (channels) or NULL */
+    const uint8_t* resets;
+    int64_t resets_b, resets_t;
+    const float* state;      /* (batch, channels, states) dense, or NULL = zeros */
+    float* state_out;        /* like state, may be `state` itself; NULL = not wanted */
+    float* marks;            /* sdfr_scan_marks_bytes() bytes: states along the way, which
+                                sdfr_scan_grad starts from; NULL where no gradient is wanted */
+    void* y;                 /* (batch, length, channels) */
+    int64_t y_b, y_t;
+    int64_t length;
+    int32_t batch, channels;
+    int32_t states;          /* 1 to 32 */
+    int32_t dtype, softplus;
+} SdfrScan;
+
+typedef struct SdfrScanGrad {
+    const void* dout;        /* gradient of y */
+    int64_t dout_b, dout_t;
+    const float* dstate_out; /* gradient of state_out, dense, or NULL */
+    void *dx, *ddt, *dz;     /* (batch, length, channels) dense; dz where there is a z */
+    void *dB, *dC;           /* (batch, length, states) dense */
+    float* dA;               /* (channels, states) */
+    float *dskip, *ddt_bias; /* (channels) or NULL */
+    float* dstate;           /* like state, or NULL */
+} SdfrScanGrad;
+
+/* `workspace`: sdfr_scan_workspace_bytes(scan, 0 or, for the gradients, 1)
+ * bytes, 64-byte aligned (0 bytes for a call of length 1 without marks). */
+SDFR_API int64_t sdfr_scan_workspace_bytes(const SdfrScan* scan, int32_t grad);
+SDFR_API int64_t sdfr_scan_marks_bytes(const SdfrScan* scan);
+SDFR_API int32_t sdfr_scan(const SdfrScan* scan, void* workspace, int64_t workspace_size,
+                           void* stream);
+/* The gradients of a call of sdfr_scan that wrote `marks` (its y and
+ * state_out are not read). */
+SDFR_API int32_t sdfr_scan_grad(const SdfrScan* scan, const SdfrScanGrad* grad, void* workspace,
+                                int64_t workspace_size, void* stream);
+
+/* One index a row, drawn from its logits. With m the largest unmasked logit
+ * and z = (x - m) / temperature, an index weighs floor(exp(z) 2^40), whole
+ * numbers, so that the answer does not go by the order of sums. Indices rank
+ * by logit, ties to the lowest; top-k keeps the first k (<= 0: all), top-p of
+ * those the ones before which less than top_p (in whole 2^-24) of their mass
+ * lies (>= 1: all), min-p of those exp(z) >= min_p. The answer is the first index at which the
+ * running sum of kept weights passes floor(u S), u being taken to 24 bits and
+ * S the sum; logp its log-probability among the kept. A temperature that is
+ * not above 0 takes the largest (lowest index, logp 0). A row with no logit
+ * above -inf gives -1 and logp 0, one with a NaN that is not masked -1 and
+ * NaN. */
+typedef struct SdfrDraw {
+    const void* logits;      /* (rows, vocab) */
+    int64_t logits_row;
+    const uint8_t* mask;     /* (rows, vocab) bytes, nonzero = legal, or NULL */
+    int64_t mask_row;
+    const float* uniform;    /* (rows), in [0, 1) */
+    const float* temperature;   /* (rows), or NULL for the one value below; likewise the others */
+    const int32_t* top_k;
+    const float *top_p, *min_p;
+    float temperature1;
+    int32_t top_k1;
+    float top_p1, min_p1;
+    int64_t* token;          /* (rows) */
+    float* logp;             /* (rows) */
+    int32_t rows, vocab;     /* vocab: 1 to 2^18 */
+    int32_t dtype;
+} SdfrDraw;
+
+SDFR_API int32_t sdfr_draw(const SdfrDraw* draw, void* stream);
+
+/* One dense tensor of a list: `size` elements from `in`, clipped into `out`
+ * (which may be `in`). */
+typedef struct SdfrTensor {
+    const void* in;
+    void* out;
+    int64_t size;
+    int32_t dtype;
+} SdfrTensor;
+
+/* norm = sqrt(sum of squares over all tensors) into *norm (device), and
+ * out = in min(1, max_norm / (norm + eps)). A norm that is not a number, or
+ * infinite, goes into the outputs as such. `tensors` is host memory;
+ * `workspace`: sdfr_clip_workspace_bytes() bytes, 8-byte aligned. */
+SDFR_API int64_t sdfr_clip_workspace_bytes(const SdfrTensor* tensors, int32_t count);
+SDFR_API int32_t sdfr_clip(const SdfrTensor* tensors, int32_t count, double max_norm, double eps,
+                           float* norm, void* workspace, int64_t workspace_size, void* stream);
+SDFR_API const char* sdfr_recurrent_last_error(void);
 
 /* Message of the calling thread's most recent error ("" if none). */
 SDFR_API const char* sdfr_last_error(void);

@@ -1,0 +1,147 @@
+"""The operators of surfgym.recurrent from their definitions, in 64 bits on the host.
+
+Loops over steps and rows, one formula after the other; the gradients are the
+formulas worked out by hand, which test_oracle_recurrent.py holds against
+differences of the forward ones.
+"""
+from __future__ import annotations
+
+import math
+
+import torch
+
+
+def _none(b, n):
+    return torch.zeros((b, n), dtype=torch.bool)
+
+
+def conv(x, weight, bias=None, *, silu=True, resets=None, state=None):
+    """(y, state); x (b, n, d), weight (d, w)."""
+    return conv_grad(x, weight, bias, silu=silu, resets=resets, state=state)[:2]
+
+
+def conv_grad(x, weight, bias=None, *, silu=True, resets=None, state=None, dy=None, dstate_out=None):
+    """(y, state, gradients by name) for the gradients dy and dstate_out (zeros)."""
+    x, w = x.double(), weight.double()
+    b, n, d = x.shape
+    width = w.shape[1]
+    r = resets.bool() if resets is not None else _none(b, n)
+    state = state.double() if state is not None else x.new_zeros((b, width - 1, d))
+    full = torch.cat([state, x], 1)                       # row t + width - 1 is step t
+    pos = torch.arange(-(width - 1), n)
+    # start[b, t]: the first position that step t may see
+    start = torch.full((b, n), -(width - 1), dtype=torch.int64)
+    cur = torch.full((b,), -(width - 1), dtype=torch.int64)
+    for t in range(n):
+        cur = torch.where(r[:, t], torch.full_like(cur, t), cur)
+        start[:, t] = cur
+    pre = torch.zeros_like(x) + (bias.double() if bias is not None else 0.0)
+    see = []
+    for j in range(width):                                # j steps back
+        rows = full[:, width - 1 - j:width - 1 - j + n]
+        m = (torch.arange(n) - j >= start)[..., None]
+        see.append(m)
+        pre = pre + torch.where(m, rows, torch.zeros_like(rows)) * w[:, width - 1 - j]
+    s = torch.sigmoid(pre)
+    y = pre * s if silu else pre
+    keep = (pos[n:][None] >= cur[:, None])[..., None]     # the last width - 1 positions
+    state_out = torch.where(keep, full[:, n:], torch.zeros_like(full[:, n:]))
+    if dy is None:
+        return y, state_out, {}
+    g = dy.double() * (s * (1 + pre * (1 - s)) if silu else 1.0)
+    dfull = torch.zeros_like(full)
+    dw = torch.zeros_like(w)
+    for j in range(width):
+        at = slice(width - 1 - j, width - 1 - j + n)
+        m = see[j].to(g.dtype)
+        dfull[:, at] += g * m * w[:, width - 1 - j]
+        dw[:, width - 1 - j] = (g * torch.where(see[j], full[:, at], torch.zeros_like(g))).sum((0, 1))
+    if dstate_out is not None:
+        dfull[:, n:] += dstate_out.double() * keep
+    return y, state_out, {"x": dfull[:, width - 1:], "state": dfull[:, :width - 1], "weight": dw,
+                          "bias": g.sum((0, 1))}
+
+
+def scan(x, dt, A, B, C, **kw):
+    """(y, state)."""
+    return scan_grad(x, dt, A, B, C, **kw)[:2]
+
+
+def scan_grad(x, dt, A, B, C, *, D=None, z=None, dt_bias=None, softplus=True, resets=None, state=None, dy=None,
+              dstate_out=None):
+    """(y, state, gradients by name) for the gradients dy and dstate_out (zeros)."""
+    x, A, B, C = x.double(), A.double(), B.double(), C.double()
+    b, n, d = x.shape
+    raw = dt.double() + (dt_bias.double() if dt_bias is not None else 0.0)
+    step = torch.logaddexp(raw, torch.zeros_like(raw)) if softplus else raw
+    skip = D.double() if D is not None else x.new_zeros(d)
+    r = resets.bool() if resets is not None else _none(b, n)
+    h = state.double().clone() if state is not None else x.new_zeros((b, d, A.shape[1]))
+    gate = z.double() * torch.sigmoid(z.double()) if z is not None else torch.ones_like(x)
+    kept, hs, core = [], [], torch.zeros_like(x)
+    decay = [torch.exp(step[:, t, :, None] * A) for t in range(n)]
+    for t in range(n):
+        past = torch.where(r[:, t, None, None], torch.zeros_like(h), h)
+        kept.append(decay[t] * past)
+        h = kept[t] + (step[:, t] * x[:, t])[..., None] * B[:, t, None, :]
+        hs.append(h)
+        core[:, t] = (h * C[:, t, None, :]).sum(-1) + skip * x[:, t]
+    y = core * gate
+    if dy is None:
+        return y, h, {}
+    dy = dy.double()
+    out = {k: torch.zeros_like(v) for k, v in (("x", x), ("dt", x), ("B", B), ("C", C), ("A", A))}
+    if z is not None:
+        s = torch.sigmoid(z.double())
+        out["z"] = dy * core * s * (1 + z.double() * (1 - s))
+    dc = dy * gate
+    g = dstate_out.double().clone() if dstate_out is not None else torch.zeros_like(h)
+    for t in range(n - 1, -1, -1):
+        g = g + dc[:, t, :, None] * C[:, t, None, :]
+        out["C"][:, t] = (dc[:, t, :, None] * hs[t]).sum(1)
+        out["B"][:, t] = (g * (step[:, t] * x[:, t])[..., None]).sum(1)
+        gb = (g * B[:, t, None, :]).sum(-1)
+        out["x"][:, t] = step[:, t] * gb + skip * dc[:, t]
+        ds = x[:, t] * gb + (g * kept[t] * A).sum(-1)
+        out["dt"][:, t] = ds * (torch.sigmoid(raw[:, t]) if softplus else 1.0)
+        out["A"] += (g * kept[t] * step[:, t, :, None]).sum(0)
+        g = torch.where(r[:, t, None, None], torch.zeros_like(g), g * decay[t])
+    out["state"] = g
+    out["D"] = (dc * x).sum((0, 1))
+    out["dt_bias"] = out["dt"].sum((0, 1))
+    return y, h, out
+
+
+def kept_probabilities(logits, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, mask=None):
+    """The distribution one row's index is drawn from (vocab,), or None where nothing may be drawn."""
+    x = logits.double()
+    if mask is not None:
+        x = torch.where(mask.bool(), x, torch.full_like(x, -math.inf))
+    v = x.numel()
+    if bool((x == -math.inf).all()):
+        return None
+    if not temperature > 0:
+        p = torch.zeros_like(x)
+        p[int((x == x.max()).nonzero()[0])] = 1.0
+        return p
+    top = x.max()
+    z = torch.where(x == top, torch.zeros_like(x), (x - top) / temperature)
+    q = torch.exp(z)
+    order = torch.sort(x, descending=True, stable=True).indices
+    kept = q[order].clone()
+    if 0 < top_k < v:
+        kept[top_k:] = 0.0
+    if top_p < 1.0:
+        before = kept.cumsum(0) - kept
+        before[0] = -1.0                                  # the likeliest stays
+        kept[before >= top_p * kept.sum()] = 0.0
+    kept[q[order] < min(min_p, 1.0)] = 0.0
+    p = torch.zeros_like(q)
+    p[order] = kept
+    return p / p.sum()
+
+
+def clip(grads, max_norm, eps=1e-6):
+    """(norm, factor)."""
+    norm = math.sqrt(sum(float((g.double() ** 2).sum()) for g in grads))
+    return norm, min(1.0, max_norm / (norm + eps))

@@ -1,0 +1,221 @@
+// clip.hip — the global 2-norm of many tensors' gradients, and their clipping:
+//
+//   norm = sqrt(sum over all elements of g^2),  g <- g min(1, max_norm / (norm + eps))
+//
+// Three steps on the stream: clip_squares leaves one partial sum a block,
+// clip_norm adds them up in a fixed order and writes the norm and the factor,
+// clip_scale multiplies. Squares and sums are fp64: no square of an fp32 value
+// overflows, and the memory is what bounds it either way.
+//
+// The tensors' addresses travel in the kernel arguments, so a call keeps
+// nothing on the device and can be captured.
+
+#include "recurrent.h"
+
+namespace {
+
+constexpr int kTensors = 96;       // of one launch: 96 * 29 bytes of kernel arguments
+constexpr int kThreads = 256;
+
+struct ClipTable {
+    const void* in[kTensors];
+    void* out[kTensors];
+    int64_t size[kTensors];
+    uint32_t first[kTensors + 1];  // the first block of each tensor
+    uint8_t dtype[kTensors];
+    int32_t count;
+    int32_t chunk;                 // elements a block takes
+};
+
+struct Span {
+    const void* in;
+    void* out;
+    int64_t from;
+    int n, dtype;
+};
+
+__device__ inline Span span_of(const ClipTable& t) {
+    int lo = 0, hi = t.count;      // the last tensor whose first block is not past this one
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        if (t.first[mid] <= blockIdx.x)
+            lo = mid;
+        else
+            hi = mid;
+    }
+    Span s;
+    s.in = t.in[lo];
+    s.out = t.out[lo];
+    s.dtype = t.dtype[lo];
+    s.from = (int64_t)(blockIdx.x - t.first[lo]) * t.chunk;
+    const int64_t left = t.size[lo] - s.from;
+    s.n = left < t.chunk ? (int)left : t.chunk;
+    return s;
+}
+
+template <typename T>
+__device__ inline double squares(const Span& s) {
+    constexpr int V = 16 / sizeof(T);
+    const T* p = (const T*)s.in + s.from;
+    double sum = 0.0;
+    const int whole = s.n / V * V;
+    for (int i = threadIdx.x * V; i < whole; i += kThreads * V) {
+        T r[V];
+        __builtin_memcpy(r, p + i, sizeof r);
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const double v = (double)(float)r[j];
+            sum = __builtin_fma(v, v, sum);
+        }
+    }
+    for (int i = whole + threadIdx.x; i < s.n; i += kThreads) {
+        const double v = (double)(float)p[i];
+        sum = __builtin_fma(v, v, sum);
+    }
+    return sum;
+}
+
+__device__ inline double block_sum(double v, double* lds) {
+#pragma unroll
+    for (int m = 32; m > 0; m /= 2) v += __shfl_xor(v, m);
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x / 64] = v;
+    __syncthreads();
+    double s = 0.0;
+    for (int j = 0; j < (int)blockDim.x / 64; ++j) s += lds[j];
+    return s;
+}
+
+__global__ __launch_bounds__(kThreads) void clip_squares(ClipTable t, double* parts) {
+    __shared__ double lds[kThreads / 64];
+    const Span s = span_of(t);
+    const double v = s.dtype == SDFR_F32 ? squares<float>(s) : s.dtype == SDFR_F16 ? squares<_Float16>(s)
+                                                                                  : squares<__bf16>(s);
+    const double sum = block_sum(v, lds);
+    if (threadIdx.x == 0) parts[blockIdx.x] = sum;
+}
+
+__global__ __launch_bounds__(1024) void clip_norm(const double* parts, int64_t count, double max_norm, double eps,
+                                                  float* norm, float* factor) {
+    __shared__ double lds[16];
+    double v = 0.0;
+    for (int64_t i = threadIdx.x; i < count; i += 1024) v += parts[i];
+    const double sum = block_sum(v, lds);
+    if (threadIdx.x != 0) return;
+    const double n = sqrt(sum), r = max_norm / (n + eps);
+    *norm = (float)n;
+    *factor = r >= 1.0 ? 1.0f : (float)r;   // a norm that is not a number leaves none behind
+}
+
+template <typename T>
+__device__ inline void scale(const Span& s, float f) {
+    constexpr int V = 16 / sizeof(T);
+    const T* p = (const T*)s.in + s.from;
+    T* q = (T*)s.out + s.from;
+    const int whole = s.n / V * V;
+    for (int i = threadIdx.x * V; i < whole; i += kThreads * V) {
+        T r[V];
+        __builtin_memcpy(r, p + i, sizeof r);
+#pragma unroll
+        for (int j = 0; j < V; ++j) r[j] = (T)((float)r[j] * f);
+        __builtin_memcpy(q + i, r, sizeof r);
+    }
+    for (int i = whole + threadIdx.x; i < s.n; i += kThreads) q[i] = (T)((float)p[i] * f);
+}
+
+__global__ __launch_bounds__(kThreads) void clip_scale(ClipTable t, const float* factor) {
+    const Span s = span_of(t);
+    const float f = *factor;
+    if (f == 1.0f && s.in == s.out) return;   // in place and within the norm: nothing changes
+    if (s.dtype == SDFR_F32)
+        scale<float>(s, f);
+    else if (s.dtype == SDFR_F16)
+        scale<_Float16>(s, f);
+    else
+        scale<__bf16>(s, f);
+}
+
+// Elements a block takes: enough blocks to fill the machine, few enough that
+// their partial sums are quickly added up.
+int chunk_of(const SdfrTensor* t, int32_t count) {
+    int64_t total = 0;
+    for (int32_t i = 0; i < count; ++i) total += t[i].size;
+    int64_t c = (total / 2048 + 4095) / 4096 * 4096;
+    return (int)(c < 4096 ? 4096 : c > 65536 ? 65536 : c);
+}
+
+int64_t blocks_of(const SdfrTensor* t, int32_t count, int chunk) {
+    int64_t blocks = 0;
+    for (int32_t i = 0; i < count; ++i) blocks += (t[i].size + chunk - 1) / chunk;
+    return blocks;
+}
+
+int32_t check_clip(const char* fn, const SdfrTensor* t, int32_t count) {
+    g_rec_err[0] = '\0';
+    if (count < 0) return rec_fail(-2, "%s: negative count", fn);
+    if (count > 0 && !t) return rec_fail(-1, "%s: null tensors", fn);
+    for (int32_t i = 0; i < count; ++i) {
+        if (t[i].size < 0 || t[i].size > ((int64_t)1 << 40)) return rec_fail(-2, "%s: bad size of tensor %d", fn, i);
+        if (!rec_float(t[i].dtype)) return rec_fail(-3, "%s: dtype of tensor %d must be f32, f16 or bf16", fn, i);
+        if (t[i].size > 0 && (!t[i].in || !t[i].out)) return rec_fail(-1, "%s: tensor %d is null", fn, i);
+    }
+    return 0;
+}
+
+}  // namespace
+
+extern "C" {
+
+SDFR_API int64_t sdfr_clip_workspace_bytes(const SdfrTensor* tensors, int32_t count) {
+    const int32_t rc = check_clip("sdfr_clip_workspace_bytes", tensors, count);
+    if (rc) return rc;
+    return 64 + blocks_of(tensors, count, chunk_of(tensors, count)) * 8;
+}
+
+SDFR_API int32_t sdfr_clip(const SdfrTensor* tensors, int32_t count, double max_norm, double eps, float* norm,
+                           void* workspace, int64_t workspace_size, void* stream) {
+    const char* fn = "sdfr_clip";
+    const int32_t rc = check_clip(fn, tensors, count);
+    if (rc) return rc;
+    if (!norm || !workspace) return rec_fail(-1, "%s: null pointer argument", fn);
+    if (!(max_norm >= 0.0) || !(eps >= 0.0)) return rec_fail(-2, "%s: max_norm and eps must not be negative", fn);
+    const int chunk = chunk_of(tensors, count);
+    const int64_t blocks = blocks_of(tensors, count, chunk);
+    if (workspace_size < 64 + blocks * 8)
+        return rec_fail(-2, "%s: workspace of %lld bytes needed (got %lld)", fn, (long long)(64 + blocks * 8),
+                        (long long)workspace_size);
+    if ((uintptr_t)workspace & 7) return rec_fail(-2, "%s: workspace must be 8-byte aligned", fn);
+    if (blocks > 0x7fffffff) return rec_fail(-2, "%s: sizes too large", fn);
+    hipStream_t st = (hipStream_t)stream;
+    float* factor = (float*)workspace;
+    double* parts = (double*)((uint8_t*)workspace + 64);
+    for (int pass = 0; pass < 2; ++pass) {
+        int64_t done = 0;
+        for (int32_t i = 0; i < count;) {
+            ClipTable t;
+            t.chunk = chunk;
+            t.count = 0;
+            uint32_t at = 0;
+            for (; i < count && t.count < kTensors; ++i) {
+                if (tensors[i].size == 0) continue;
+                const int k = t.count++;
+                t.in[k] = tensors[i].in;
+                t.out[k] = tensors[i].out;
+                t.size[k] = tensors[i].size;
+                t.dtype[k] = (uint8_t)tensors[i].dtype;
+                t.first[k] = at;
+                at += (uint32_t)((tensors[i].size + chunk - 1) / chunk);
+            }
+            if (t.count == 0) break;
+            t.first[t.count] = at;
+            if (pass == 0)
+                clip_squares<<<at, kThreads, 0, st>>>(t, parts + done);
+            else
+                clip_scale<<<at, kThreads, 0, st>>>(t, factor);
+            done += at;
+        }
+        if (pass == 0) clip_norm<<<1, 1024, 0, st>>>(parts, blocks, max_norm, eps, norm, factor);
+    }
+    return rec_launched(fn);
+}
+
+}  // extern "C"

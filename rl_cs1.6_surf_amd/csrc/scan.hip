@@ -1,0 +1,811 @@
+// scan.hip — the selective state space scan: a policy's memory over the
+// decisions of a rollout or the tokens of a prompt, its gradients, and its
+// step for a single token.
+//
+//   D[t]   = softplus(dt[t] + dt_bias)                          per channel d
+//   a[t,n] = exp(D[t] A[d,n]), 0 where a sequence begins (resets)
+//   h[t,n] = a[t,n] h[t-1,n] + D[t] x[t] B[t,n]
+//   y[t]   = sum_n C[t,n] h[t,n] + skip[d] x[t];   out = y silu(z)
+//
+// and backwards, with dy = dout silu(z),
+//
+//   g[t,n]  = dy[t] C[t,n] + a[t+1,n] g[t+1,n]
+//   dC[t,n] = sum_d dy[t] h[t,n]            dB[t,n] = sum_d g[t,n] D[t] x[t]
+//   dx[t]   = D[t] sum_n g B + skip dy      dA[n]   = sum_t g (a h[t-1]) D[t]
+//   dD[t]   = x[t] sum_n g B + sum_n g (a h[t-1]) A;  ddt = dD sigmoid(dt + dt_bias)
+//
+// Layout: a lane is a channel and holds its N states in registers; a wave
+// walks along the time of 64 channels of one sequence. Channels are the
+// innermost axis, so each step's loads are one row segment, and B[t], C[t]
+// are the same for all lanes: bc_pack lays them out once as fp32, zero padded
+// to the kernel's state count, and the walk reads them through the scalar
+// cache into SGPRs.
+//
+// Few sequences: the walk is cut into chunks that run side by side. A first
+// pass walks each chunk from zero and keeps only its end and the product of
+// its decays, scan_join strings them together, and the real pass starts every
+// chunk from its own state.
+
+#include "recurrent.h"
+
+namespace {
+
+using namespace rec;
+
+typedef const __attribute__((address_space(4))) float* uniform_f32;   // read through the scalar cache
+
+struct Rows {   // (batch, step, channel) with a unit channel stride
+    const void* p;
+    int64_t b, t;
+};
+
+struct ScanArgs {
+    Rows x, dt, z;          // z.p may be null
+    const float* bc;        // (batch, length, 2 NS) packed B, C
+    const float *A, *skip, *bias;
+    const uint8_t* resets;  // null: none
+    int64_t resets_b, resets_t;
+    const float* state;     // (batch, channels, N) or null
+    float* state_out;
+    float* marks;           // (batch, tiles, NS, channels): the state before each tile, or null
+    float *ends, *prods;    // (batch, chunks, NS, channels)
+    void* y;
+    int64_t y_b, y_t;
+    int64_t length, chunk;
+    int batch, channels, N, chunks, blocks, softplus;   // blocks: of 64 channels
+};
+
+struct GradArgs {
+    Rows dout;
+    const float* dstate_out;   // (batch, channels, N) or null
+    void *dx, *ddt, *dz;       // (batch, length, channels) dense
+    float* dstate;             // (batch, channels, N) or null
+    float* bc_part;            // (blocks, batch, length, 2 NS)
+    float* sums;               // (batch, chunks, NS + 2, channels): dA, dskip, dbias
+    float* ends;               // (batch, chunks, NS, channels): g carried into each chunk's end
+};
+
+template <int NS> constexpr int kTile = 128 / NS;   // steps whose decayed states fit 128 registers
+
+// softplus and its derivative; log1p as log(1+e) plus what 1+e rounded off.
+__device__ inline float softplus(float v) {
+    const float e = exp_near(-fabsf(v));
+    const float w = 1.0f + e;
+    const float l = __builtin_fmaf(e - (w - 1.0f), __builtin_amdgcn_rcpf(w), __builtin_amdgcn_logf(w) * kLn2);
+    return fmaxf(v, 0.0f) + l;
+}
+
+// Bit i: does a sequence begin at step t + i? (one load for 64 steps)
+__device__ inline uint64_t resets_at(const ScanArgs& a, int b, int64_t t, int64_t end) {
+    const int64_t k = t + threadIdx.x;
+    const bool r = k < end && a.resets[b * a.resets_b + k * a.resets_t] != 0;
+    return __ballot(r);
+}
+
+struct Place {
+    int b, s, blk, d;
+    bool live;
+    int64_t t0, t1;
+};
+
+__device__ inline Place place_of(const ScanArgs& a) {
+    Place p;
+    const int64_t id = blockIdx.x;
+    p.blk = (int)(id % a.blocks);
+    const int64_t r = id / a.blocks;
+    p.s = (int)(r % a.chunks);
+    p.b = (int)(r / a.chunks);
+    const int d = p.blk * 64 + threadIdx.x;
+    p.live = d < a.channels;
+    p.d = p.live ? d : a.channels - 1;   // lanes past the end repeat the last channel and write nothing
+    p.t0 = p.s * a.chunk;
+    p.t1 = p.t0 + a.chunk < a.length ? p.t0 + a.chunk : a.length;
+    return p;
+}
+
+template <int NS>
+__device__ inline void load_rates(const ScanArgs& a, int d, float (&A2)[NS]) {
+#pragma unroll
+    for (int n = 0; n < NS; ++n) A2[n] = n < a.N ? a.A[(int64_t)d * a.N + n] * kLog2e : 0.0f;
+}
+
+// ---- packing B and C -------------------------------------------------------
+template <typename T, int NS>
+__global__ __launch_bounds__(256) void bc_pack(Rows B, Rows C, float* __restrict__ bc, int64_t rows, int64_t length,
+                                               int N) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t row = i / (2 * NS);
+    const int k = (int)(i % (2 * NS)), n = k % NS;
+    if (row >= rows) return;
+    const int64_t b = row / length, t = row % length;
+    const Rows& r = k < NS ? B : C;
+    bc[i] = n < N ? (float)((const T*)r.p)[b * r.b + t * r.t + n] : 0.0f;
+}
+
+// ---- forward ---------------------------------------------------------------
+// ENDS: only the chunk's end state from zero and the product of its decays.
+template <typename T, int NS, bool ENDS>
+__global__ __launch_bounds__(64) void scan_forward(ScanArgs a) {
+    constexpr int TT = 8;
+    const Place p = place_of(a);
+    float A2[NS], h[NS];
+    load_rates<NS>(a, p.d, A2);
+    const int64_t slot = (((int64_t)p.b * a.chunks + p.s) * NS) * a.channels + p.d;
+#pragma unroll
+    for (int n = 0; n < NS; ++n) {
+        if (ENDS)
+            h[n] = 0.0f;
+        else if (a.chunks > 1)
+            h[n] = a.ends[slot + (int64_t)n * a.channels];
+        else
+            h[n] = a.state && n < a.N ? a.state[((int64_t)p.b * a.channels + p.d) * a.N + n] : 0.0f;
+    }
+    const float skip = a.skip ? a.skip[p.d] : 0.0f, bias = a.bias ? a.bias[p.d] : 0.0f;
+    const T* xp = (const T*)a.x.p + p.b * a.x.b + p.d;
+    const T* dp = (const T*)a.dt.p + p.b * a.dt.b + p.d;
+    const bool gated = !ENDS && a.z.p;
+    const T* zp = gated ? (const T*)a.z.p + p.b * a.z.b + p.d : xp;
+    T* yp = ENDS ? nullptr : (T*)a.y + p.b * a.y_b + p.d;
+    const uniform_f32 bc = (uniform_f32)(uintptr_t)(a.bc + (int64_t)p.b * a.length * 2 * NS);
+    uint64_t starts = 0;
+    bool cut = false;
+    float sum = 0.0f;
+    T xr[TT], dr[TT], zr[TT];
+    auto fetch = [&](int64_t t) {
+#pragma unroll
+        for (int i = 0; i < TT; ++i) {
+            const int64_t k = t + i < p.t1 ? t + i : p.t1 - 1;
+            xr[i] = xp[k * a.x.t];
+            dr[i] = dp[k * a.dt.t];
+            if (gated) zr[i] = zp[k * a.z.t];
+        }
+    };
+    fetch(p.t0);
+    for (int64_t t = p.t0; t < p.t1; t += TT) {
+        if (a.resets && ((t - p.t0) & 63) == 0) starts = resets_at(a, p.b, t, p.t1);
+        float x[TT], dl[TT], z[TT];
+#pragma unroll
+        for (int i = 0; i < TT; ++i) {
+            x[i] = (float)xr[i];
+            dl[i] = (float)dr[i] + bias;
+            z[i] = gated ? (float)zr[i] : 0.0f;
+        }
+        if (t + TT < p.t1) fetch(t + TT);
+#pragma unroll
+        for (int i = 0; i < TT; ++i) {
+            if (t + i >= p.t1) break;
+            const uniform_f32 row = bc + (t + i) * 2 * NS;
+            if (a.softplus) dl[i] = softplus(dl[i]);
+            if (starts & 1) {
+                cut = true;
+#pragma unroll
+                for (int n = 0; n < NS; ++n) h[n] = 0.0f;
+            }
+            starts >>= 1;
+            if (!ENDS && a.marks && (t + i) % kTile<NS> == 0 && p.live) {
+                float* m = a.marks + (((int64_t)p.b * ((a.length + kTile<NS> - 1) / kTile<NS>) + (t + i) / kTile<NS>) * NS) *
+                                         a.channels + p.d;
+#pragma unroll
+                for (int n = 0; n < NS; ++n) m[(int64_t)n * a.channels] = h[n];
+            }
+            const float in = dl[i] * x[i];
+            if (ENDS) sum += dl[i];
+            float y0 = skip * x[i], y1 = 0.0f;
+#pragma unroll
+            for (int n = 0; n < NS; ++n) {
+                h[n] = __builtin_fmaf(exp2_fast(dl[i] * A2[n]), h[n], in * row[n]);
+                if (!ENDS) {
+                    if (n & 1)
+                        y1 = __builtin_fmaf(h[n], row[NS + n], y1);
+                    else
+                        y0 = __builtin_fmaf(h[n], row[NS + n], y0);
+                }
+            }
+            if (!ENDS) {
+                float y = y0 + y1;
+                if (gated) y *= z[i] * sigmoid(z[i]);
+                if (p.live) yp[(t + i) * a.y_t] = (T)y;
+            }
+        }
+    }
+    if (!p.live) return;
+    if (ENDS) {
+#pragma unroll
+        for (int n = 0; n < NS; ++n) {
+            a.ends[slot + (int64_t)n * a.channels] = h[n];
+            a.prods[slot + (int64_t)n * a.channels] = cut ? 0.0f : exp2_fast(sum * A2[n]);
+        }
+    } else if (a.state_out && p.t1 == a.length) {
+#pragma unroll
+        for (int n = 0; n < NS; ++n)
+            if (n < a.N) a.state_out[((int64_t)p.b * a.channels + p.d) * a.N + n] = h[n];
+    }
+}
+
+// Strings the chunks together in place: ends[s] becomes what chunk s starts
+// from. Backwards (REV) the order turns round and the seed is the gradient of
+// the final state.
+template <bool REV>
+__global__ __launch_bounds__(256) void scan_join(float* ends, const float* prods, const float* seed, int batch,
+                                                 int chunks, int NS, int channels, int N) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t row = (int64_t)NS * channels;
+    if (i >= batch * row) return;
+    const int64_t b = i / row, r = i % row;
+    const int n = (int)(r / channels), d = (int)(r % channels);
+    float carry = seed && n < N ? seed[(b * channels + d) * N + n] : 0.0f;
+    float* e = ends + b * chunks * row + r;
+    const float* q = prods + b * chunks * row + r;
+    for (int k = 0; k < chunks; ++k) {
+        const int64_t s = (REV ? chunks - 1 - k : k) * row;
+        const float end = e[s], prod = q[s];
+        e[s] = carry;
+        carry = prod == 0.0f ? end : __builtin_fmaf(prod, carry, end);   // a cut keeps nothing, not even a NaN
+    }
+}
+
+// ---- backward --------------------------------------------------------------
+// Sums over the 64 lanes of 64 values a lane, folded in pairs: at every level
+// a lane keeps one of two values and takes its partner's share of it, so a
+// value costs about two instructions instead of six. Level j pairs values
+// whose index differs in bit j and lanes that differ in bit 5 - j.
+template <int LEVEL>
+__device__ inline float fold(float a, float b) {
+    const unsigned ua = __float_as_uint(a), ub = __float_as_uint(b);
+    if constexpr (LEVEL == 0) {
+        const auto r = __builtin_amdgcn_permlane32_swap(ua, ub, false, false);
+        return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    } else if constexpr (LEVEL == 1) {
+        const auto r = __builtin_amdgcn_permlane16_swap(ua, ub, false, false);
+        return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    } else {
+        // partners: 8 apart, mirrored in 8 lanes, 2 apart, 1 apart
+        constexpr int ctrl = LEVEL == 2 ? 0x128 : LEVEL == 3 ? 0x141 : LEVEL == 4 ? 0x4E : 0xB1;
+        const bool hi = threadIdx.x & (32 >> LEVEL);
+        const float keep = hi ? b : a, give = hi ? a : b;
+        const int got = __builtin_amdgcn_update_dpp(0, __float_as_int(give), ctrl, 0xf, 0xf, true);
+        return keep + __int_as_float(got);
+    }
+}
+
+template <int LEVEL, int COUNT>
+__device__ inline float fold_all(float (&v)[COUNT]) {
+    if constexpr (COUNT == 1) {
+        return v[0];
+    } else {
+        float r[COUNT / 2];
+#pragma unroll
+        for (int i = 0; i < COUNT / 2; ++i) r[i] = fold<LEVEL>(v[2 * i], v[2 * i + 1]);
+        return fold_all<LEVEL + 1>(r);
+    }
+}
+
+constexpr int log2_of(int v) { return v <= 1 ? 0 : 1 + log2_of(v / 2); }
+
+// A chunk's g carried out of its start, from zero, and the product of its decays.
+template <typename T, int NS>
+__global__ __launch_bounds__(64) void scan_backward_ends(ScanArgs a, GradArgs ga) {
+    const Place p = place_of(a);
+    float A2[NS], g[NS];
+    load_rates<NS>(a, p.d, A2);
+#pragma unroll
+    for (int n = 0; n < NS; ++n) g[n] = 0.0f;
+    const float bias = a.bias ? a.bias[p.d] : 0.0f;
+    const T* dp = (const T*)a.dt.p + p.b * a.dt.b + p.d;
+    const T* op = (const T*)ga.dout.p + p.b * ga.dout.b + p.d;
+    const T* zp = a.z.p ? (const T*)a.z.p + p.b * a.z.b + p.d : nullptr;
+    const uniform_f32 bc = (uniform_f32)(uintptr_t)(a.bc + (int64_t)p.b * a.length * 2 * NS);
+    float sum = 0.0f;
+    bool cut = false;
+    uint64_t starts = 0;
+    int64_t from = p.t1;   // first step that `starts` speaks of
+    for (int64_t t = p.t1 - 1; t >= p.t0; --t) {
+        if (a.resets && t < from) {
+            from = p.t0 + (t - p.t0) / 64 * 64;
+            starts = resets_at(a, p.b, from, p.t1);
+        }
+        float dl = (float)dp[t * a.dt.t] + bias;
+        if (a.softplus) dl = softplus(dl);
+        float dy = (float)op[t * ga.dout.t];
+        if (zp) {
+            const float z = (float)zp[t * a.z.t];
+            dy *= z * sigmoid(z);
+        }
+        const uniform_f32 row = bc + t * 2 * NS + NS;
+        sum += dl;
+#pragma unroll
+        for (int n = 0; n < NS; ++n) g[n] = __builtin_fmaf(dy, row[n], g[n]) * exp2_fast(dl * A2[n]);
+        if (starts >> (t - from) & 1) {
+            cut = true;
+#pragma unroll
+            for (int n = 0; n < NS; ++n) g[n] = 0.0f;
+        }
+    }
+    if (!p.live) return;
+    const int64_t slot = (((int64_t)p.b * a.chunks + p.s) * NS) * a.channels + p.d;
+#pragma unroll
+    for (int n = 0; n < NS; ++n) {
+        ga.ends[slot + (int64_t)n * a.channels] = g[n];
+        a.prods[slot + (int64_t)n * a.channels] = cut ? 0.0f : exp2_fast(sum * A2[n]);
+    }
+}
+
+template <typename T, int NS>
+__global__ __launch_bounds__(64, 2) void scan_backward(ScanArgs a, GradArgs ga) {
+    constexpr int TT = kTile<NS>;
+    constexpr int G = 64 / (2 * NS);   // steps whose 2 NS sums fill the lanes
+    const Place p = place_of(a);
+    float A2[NS], g[NS], dA[NS];
+    load_rates<NS>(a, p.d, A2);
+    const int64_t slot = (((int64_t)p.b * a.chunks + p.s) * NS) * a.channels + p.d;
+#pragma unroll
+    for (int n = 0; n < NS; ++n) {
+        dA[n] = 0.0f;
+        if (a.chunks > 1)
+            g[n] = ga.ends[slot + (int64_t)n * a.channels];
+        else
+            g[n] = ga.dstate_out && n < a.N ? ga.dstate_out[((int64_t)p.b * a.channels + p.d) * a.N + n] : 0.0f;
+    }
+    const float skip = a.skip ? a.skip[p.d] : 0.0f, bias = a.bias ? a.bias[p.d] : 0.0f;
+    float dskip = 0.0f, dbias = 0.0f;
+    const T* xp = (const T*)a.x.p + p.b * a.x.b + p.d;
+    const T* dp = (const T*)a.dt.p + p.b * a.dt.b + p.d;
+    const T* op = (const T*)ga.dout.p + p.b * ga.dout.b + p.d;
+    const bool gated = a.z.p != nullptr;
+    const T* zp = gated ? (const T*)a.z.p + p.b * a.z.b + p.d : xp;
+    const int64_t dense = (int64_t)p.b * a.length * a.channels + p.d;
+    T* dxp = (T*)ga.dx + dense;
+    T* ddp = (T*)ga.ddt + dense;
+    T* dzp = gated ? (T*)ga.dz + dense : nullptr;
+    const uniform_f32 bc = (uniform_f32)(uintptr_t)(a.bc + (int64_t)p.b * a.length * 2 * NS);
+    const int64_t tiles = (a.length + TT - 1) / TT;
+    // the sums' place: lane l ends up with the value whose index is l's bits turned round
+    const int k = (int)(__builtin_bitreverse32(threadIdx.x) >> 26);
+    float* part = ga.bc_part + (((int64_t)p.blk * a.batch + p.b) * a.length + k / (2 * NS)) * 2 * NS + k % (2 * NS);
+    uint64_t starts = 0;
+    int64_t from = p.t1;
+
+    for (int64_t t = p.t0 + (p.t1 - 1 - p.t0) / TT * TT; t >= p.t0; t -= TT) {
+        if (a.resets && t < from) {
+            from = p.t0 + (t - p.t0) / 64 * 64;
+            starts = resets_at(a, p.b, from, p.t1);
+        }
+        const unsigned cuts = (unsigned)(starts >> (t - from));
+        float w[TT][NS], dl[TT], x[TT], dy[TT], sg[TT];
+        float h[NS];
+        const float* m = a.marks + (((int64_t)p.b * tiles + t / TT) * NS) * a.channels + p.d;
+#pragma unroll
+        for (int n = 0; n < NS; ++n) h[n] = m[(int64_t)n * a.channels];
+        // forwards through the tile: w = what each step keeps of its past.
+        // Steps past the end are steps of nothing: D = 0, x = 0, dy = 0.
+#pragma unroll
+        for (int i = 0; i < TT; ++i) {
+            const bool in = t + i < p.t1;
+            const int64_t q = in ? t + i : p.t1 - 1;
+            const uniform_f32 row = bc + q * 2 * NS;
+            float v = (float)dp[q * a.dt.t] + bias;
+            sg[i] = a.softplus ? sigmoid(v) : 1.0f;
+            if (a.softplus) v = softplus(v);
+            dl[i] = in ? v : 0.0f;
+            x[i] = in ? (float)xp[q * a.x.t] : 0.0f;
+            const float dout = in ? (float)op[q * ga.dout.t] : 0.0f;
+            const float u = dl[i] * x[i];
+            if (cuts >> i & 1) {
+#pragma unroll
+                for (int n = 0; n < NS; ++n) h[n] = 0.0f;
+            }
+            float y0 = skip * x[i], y1 = 0.0f;
+#pragma unroll
+            for (int n = 0; n < NS; ++n) {
+                w[i][n] = exp2_fast(dl[i] * A2[n]) * h[n];
+                h[n] = __builtin_fmaf(u, row[n], w[i][n]);
+                if (gated) {
+                    if (n & 1)
+                        y1 = __builtin_fmaf(h[n], row[NS + n], y1);
+                    else
+                        y0 = __builtin_fmaf(h[n], row[NS + n], y0);
+                }
+            }
+            dy[i] = dout;
+            if (gated) {
+                const float z = (float)zp[q * a.z.t], s = sigmoid(z);
+                dy[i] = dout * z * s;
+                if (in && p.live) dzp[q * a.channels] = (T)(dout * (y0 + y1) * s * __builtin_fmaf(z, 1.0f - s, 1.0f));
+            }
+        }
+        float r[G];
+#pragma unroll
+        for (int i = TT - 1; i >= 0; --i) {
+            const bool in = t + i < p.t1;
+            const int64_t q = in ? t + i : p.t1 - 1;
+            const uniform_f32 row = bc + q * 2 * NS;
+            const float u = dl[i] * x[i];
+            float v[2 * NS], gb = 0.0f, ga_ = 0.0f;
+#pragma unroll
+            for (int n = 0; n < NS; ++n) {
+                g[n] = __builtin_fmaf(dy[i], row[NS + n], g[n]);
+                v[n] = p.live ? g[n] * u : 0.0f;
+                v[NS + n] = p.live ? dy[i] * __builtin_fmaf(u, row[n], w[i][n]) : 0.0f;
+                gb = __builtin_fmaf(g[n], row[n], gb);
+                const float kept = g[n] * w[i][n];
+                ga_ = __builtin_fmaf(kept, A2[n], ga_);
+                dA[n] = __builtin_fmaf(kept, dl[i], dA[n]);
+                g[n] *= exp2_fast(dl[i] * A2[n]);
+            }
+            if (cuts >> i & 1) {
+#pragma unroll
+                for (int n = 0; n < NS; ++n) g[n] = 0.0f;
+            }
+            const float ddl = __builtin_fmaf(x[i], gb, ga_ * kLn2) * sg[i];
+            if (in) {
+                dskip = __builtin_fmaf(dy[i], x[i], dskip);
+                dbias += ddl;
+                if (p.live) {
+                    dxp[q * a.channels] = (T)__builtin_fmaf(dl[i], gb, skip * dy[i]);
+                    ddp[q * a.channels] = (T)ddl;
+                }
+            }
+            r[i % G] = fold_all<0>(v);
+            if (i % G == 0) {
+                const float s = fold_all<log2_of(2 * NS)>(r);
+                if (t + i + k / (2 * NS) < p.t1) part[(t + i) * 2 * NS] = s;
+            }
+        }
+    }
+    if (!p.live) return;
+    float* sums = ga.sums + (((int64_t)p.b * a.chunks + p.s) * (NS + 2)) * a.channels + p.d;
+#pragma unroll
+    for (int n = 0; n < NS; ++n) sums[(int64_t)n * a.channels] = dA[n];
+    sums[(int64_t)NS * a.channels] = dskip;
+    sums[(int64_t)(NS + 1) * a.channels] = dbias;
+    if (ga.dstate && p.s == 0) {
+#pragma unroll
+        for (int n = 0; n < NS; ++n)
+            if (n < a.N) ga.dstate[((int64_t)p.b * a.channels + p.d) * a.N + n] = g[n];
+    }
+}
+
+// dB and dC from the blocks' partial sums, always in the same order.
+template <typename T, int NS>
+__global__ __launch_bounds__(256) void bc_sums(const float* __restrict__ part, T* __restrict__ dB, T* __restrict__ dC,
+                                               int64_t rows, int blocks, int N) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t size = rows * 2 * NS;
+    if (i >= size) return;
+    const int k = (int)(i % (2 * NS)), n = k % NS;
+    if (n >= N) return;
+    float s = 0.0f;
+    for (int j = 0; j < blocks; ++j) s += part[j * size + i];
+    (k < NS ? dB : dC)[i / (2 * NS) * N + n] = (T)s;
+}
+
+// dA, dskip and dbias from the walks' sums: 64 columns a block, 16 shares of
+// the rows, always in the same order.
+__global__ __launch_bounds__(1024) void column_sums(const float* __restrict__ sums, float* dA, float* dskip,
+                                                    float* dbias, int64_t rows, int NS, int channels, int N) {
+    __shared__ float lds[16][64];
+    const int64_t cols = (int64_t)(NS + 2) * channels;
+    const int64_t c = (int64_t)blockIdx.x * 64 + threadIdx.x;
+    float s = 0.0f;
+    if (c < cols)
+        for (int64_t r = threadIdx.y; r < rows; r += 16) s += sums[r * cols + c];
+    lds[threadIdx.y][threadIdx.x] = s;
+    __syncthreads();
+    if (threadIdx.y != 0 || c >= cols) return;
+    for (int j = 1; j < 16; ++j) s += lds[j][threadIdx.x];
+    const int n = (int)(c / channels), d = (int)(c % channels);
+    if (n < N) {
+        dA[(int64_t)d * N + n] = s;
+    } else if (n == NS) {
+        if (dskip) dskip[d] = s;
+    } else if (n == NS + 1) {
+        if (dbias) dbias[d] = s;
+    }
+}
+
+// ---- a single token ----------------------------------------------------------
+// What bounds it is the state, read and written once: a lane takes four states
+// of a channel (one 16-byte load and store), LANES lanes a channel, and the sum
+// over states is folded over those lanes.
+template <typename T, int LANES, bool WIDE>
+__global__ __launch_bounds__(256) void scan_step(ScanArgs a, Rows B, Rows C) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t c = i / LANES;
+    const int n0 = (int)(i % LANES) * 4;
+    const bool live = c < (int64_t)a.batch * a.channels;
+    const int64_t cc = live ? c : 0;
+    const int64_t b = cc / a.channels;
+    const int d = (int)(cc % a.channels);
+    float h[4], A[4], Bn[4], Cn[4];
+    const int64_t at = cc * a.N + n0, rate = (int64_t)d * a.N + n0;
+    const T* Bp = (const T*)B.p + b * B.b + n0;
+    const T* Cp = (const T*)C.p + b * C.b + n0;
+    if (WIDE) {
+        const float4 v = a.state ? *(const float4*)(a.state + at) : float4{0, 0, 0, 0};
+        const float4 r = *(const float4*)(a.A + rate);
+        h[0] = v.x, h[1] = v.y, h[2] = v.z, h[3] = v.w;
+        A[0] = r.x, A[1] = r.y, A[2] = r.z, A[3] = r.w;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) Bn[j] = (float)Bp[j], Cn[j] = (float)Cp[j];
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const bool in = n0 + j < a.N;
+            h[j] = in && a.state ? a.state[at + j] : 0.0f;
+            A[j] = in ? a.A[rate + j] : 0.0f;
+            Bn[j] = in ? (float)Bp[j] : 0.0f;
+            Cn[j] = in ? (float)Cp[j] : 0.0f;
+        }
+    }
+    const float x = (float)((const T*)a.x.p)[b * a.x.b + d];
+    float dl = (float)((const T*)a.dt.p)[b * a.dt.b + d] + (a.bias ? a.bias[d] : 0.0f);
+    if (a.softplus) dl = softplus(dl);
+    const bool begins = a.resets && a.resets[b * a.resets_b] != 0;
+    const float in = dl * x;
+    float y = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        if (begins) h[j] = 0.0f;
+        h[j] = __builtin_fmaf(exp2_fast(dl * (A[j] * kLog2e)), h[j], in * Bn[j]);
+        y = __builtin_fmaf(h[j], Cn[j], y);
+    }
+#pragma unroll
+    for (int m = 1; m < LANES; m *= 2) y += __shfl_xor(y, m);
+    if (!live) return;
+    if (a.state_out) {
+        if (WIDE) {
+            *(float4*)(a.state_out + at) = float4{h[0], h[1], h[2], h[3]};
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (n0 + j < a.N) a.state_out[at + j] = h[j];
+        }
+    }
+    if (n0 != 0) return;
+    if (a.skip) y = __builtin_fmaf(a.skip[d], x, y);
+    if (a.z.p) {
+        const float z = (float)((const T*)a.z.p)[b * a.z.b + d];
+        y *= z * sigmoid(z);
+    }
+    ((T*)a.y)[b * a.y_b + d] = (T)y;
+}
+
+// ---- host --------------------------------------------------------------------
+constexpr int kMaxStates = 32;
+
+int padded(int n) { return n <= 8 ? 8 : n <= 16 ? 16 : 32; }
+
+struct Plan {
+    int NS, blocks, chunks;
+    int64_t chunk, bc, ends, part, sums, total;   // byte offsets of the workspace's parts
+};
+
+// Cuts the time where the sequences alone do not fill the machine (1024 SIMDs).
+Plan plan_of(const SdfrScan* s, bool grad) {
+    Plan p;
+    p.NS = padded(s->states);
+    p.blocks = (s->channels + 63) / 64;
+    const int64_t waves = (int64_t)s->batch * p.blocks;
+    int64_t chunks = 1;
+    if (waves < 1024) chunks = (2048 + waves - 1) / waves;
+    const int64_t most = s->length / 32;
+    if (chunks > most) chunks = most < 1 ? 1 : most;
+    p.chunk = ((s->length + chunks - 1) / chunks + 15) / 16 * 16;
+    p.chunks = (int)((s->length + p.chunk - 1) / p.chunk);
+    auto up = [](int64_t v) { return (v + 255) & ~(int64_t)255; };
+    const int64_t rows = (int64_t)s->batch * s->length;
+    const int64_t ends = p.chunks > 1 ? (int64_t)s->batch * p.chunks * p.NS * s->channels * 4 : 0;
+    p.bc = 0;
+    p.ends = up(rows * 2 * p.NS * 4);
+    p.part = p.ends + 2 * up(ends);
+    p.sums = p.part + (grad ? up(rows * 2 * p.NS * 4 * p.blocks) : 0);
+    p.total = p.sums + (grad ? up((int64_t)s->batch * p.chunks * (p.NS + 2) * s->channels * 4) : 0);
+    return p;
+}
+
+int32_t check_scan(const char* fn, const SdfrScan* s) {
+    g_rec_err[0] = '\0';
+    if (!s) return rec_fail(-1, "%s: null descriptor", fn);
+    if (s->batch < 0 || s->length < 0 || s->channels < 1)
+        return rec_fail(-2, "%s: bad sizes (batch %d, length %lld, channels %d)", fn, s->batch, (long long)s->length,
+                        s->channels);
+    if (s->states < 1 || s->states > kMaxStates)
+        return rec_fail(-2, "%s: states must be 1 to %d (got %d)", fn, kMaxStates, s->states);
+    if (!rec_float(s->dtype)) return rec_fail(-3, "%s: dtype must be f32, f16 or bf16 (got %d)", fn, s->dtype);
+    if (s->channels > (1 << 24) || s->length > ((int64_t)1 << 40) ||
+        (int64_t)s->batch * ((s->channels + 63) / 64) > 0x3fffffff)
+        return rec_fail(-2, "%s: sizes too large", fn);
+    if (!s->A) return rec_fail(-1, "%s: null rates", fn);
+    if (s->batch > 0 && s->length > 0 && (!s->x || !s->dt || !s->B || !s->C || !s->y))
+        return rec_fail(-1, "%s: null pointer argument", fn);
+    return 0;
+}
+
+ScanArgs args_of(const SdfrScan* s, const Plan& p, uint8_t* ws) {
+    ScanArgs a;
+    memset(&a, 0, sizeof a);
+    a.x = {s->x, s->x_b, s->x_t};
+    a.dt = {s->dt, s->dt_b, s->dt_t};
+    a.z = {s->z, s->z_b, s->z_t};
+    a.A = s->A;
+    a.skip = s->skip;
+    a.bias = s->dt_bias;
+    a.resets = s->resets;
+    a.resets_b = s->resets_b;
+    a.resets_t = s->resets_t;
+    a.state = s->state;
+    a.state_out = s->state_out;
+    a.marks = s->marks;
+    a.y = s->y;
+    a.y_b = s->y_b;
+    a.y_t = s->y_t;
+    a.length = s->length;
+    a.chunk = p.chunk;
+    a.batch = s->batch;
+    a.channels = s->channels;
+    a.N = s->states;
+    a.chunks = p.chunks;
+    a.blocks = p.blocks;
+    a.softplus = s->softplus;
+    if (ws) {
+        a.bc = (const float*)(ws + p.bc);
+        a.ends = (float*)(ws + p.ends);
+        a.prods = a.ends + (int64_t)s->batch * p.chunks * p.NS * s->channels;
+    }
+    return a;
+}
+
+template <class F>
+int32_t with_states(int NS, F f) {
+    if (NS == 8) return f(std::integral_constant<int, 8>());
+    if (NS == 16) return f(std::integral_constant<int, 16>());
+    return f(std::integral_constant<int, 32>());
+}
+
+int32_t check_workspace(const char* fn, const Plan& p, void* ws, int64_t size) {
+    if (!ws) return rec_fail(-1, "%s: null workspace", fn);
+    if (size < p.total)
+        return rec_fail(-2, "%s: workspace of %lld bytes needed (got %lld)", fn, (long long)p.total, (long long)size);
+    if ((uintptr_t)ws & 63) return rec_fail(-2, "%s: workspace must be 64-byte aligned", fn);
+    return 0;
+}
+
+template <typename T, int NS>
+void launch_pack(const SdfrScan* s, const ScanArgs& a, hipStream_t st) {
+    const int64_t rows = (int64_t)s->batch * s->length;
+    bc_pack<T, NS><<<(unsigned)((rows * 2 * NS + 255) / 256), 256, 0, st>>>(
+        Rows{s->B, s->B_b, s->B_t}, Rows{s->C, s->C_b, s->C_t}, (float*)a.bc, rows, s->length, s->states);
+}
+
+template <typename T, int LANES>
+void launch_step(const SdfrScan* s, const ScanArgs& a, hipStream_t st) {
+    const int64_t lanes = (int64_t)s->batch * s->channels * LANES;
+    const unsigned blocks = (unsigned)((lanes + 255) / 256);
+    const Rows B{s->B, s->B_b, s->B_t}, C{s->C, s->C_b, s->C_t};
+    const bool wide = s->states == LANES * 4 && !(((uintptr_t)s->state | (uintptr_t)s->state_out | (uintptr_t)s->A) & 15);
+    if (wide)
+        scan_step<T, LANES, true><<<blocks, 256, 0, st>>>(a, B, C);
+    else
+        scan_step<T, LANES, false><<<blocks, 256, 0, st>>>(a, B, C);
+}
+
+}  // namespace
+
+extern "C" {
+
+SDFR_API const char* sdfr_recurrent_last_error(void) { return g_rec_err; }
+
+SDFR_API int64_t sdfr_scan_workspace_bytes(const SdfrScan* s, int32_t grad) {
+    const int32_t rc = check_scan("sdfr_scan_workspace_bytes", s);
+    if (rc) return rc;
+    if (s->batch == 0 || s->length == 0 || (!grad && s->length == 1 && !s->marks)) return 0;
+    return plan_of(s, grad != 0).total;
+}
+
+SDFR_API int64_t sdfr_scan_marks_bytes(const SdfrScan* s) {
+    const int32_t rc = check_scan("sdfr_scan_marks_bytes", s);
+    if (rc) return rc;
+    const int NS = padded(s->states), tile = 128 / NS;
+    return (int64_t)s->batch * ((s->length + tile - 1) / tile) * NS * s->channels * 4;
+}
+
+SDFR_API int32_t sdfr_scan(const SdfrScan* s, void* workspace, int64_t workspace_size, void* stream) {
+    const char* fn = "sdfr_scan";
+    int32_t rc = check_scan(fn, s);
+    if (rc) return rc;
+    if (s->batch == 0) return 0;
+    hipStream_t st = (hipStream_t)stream;
+    if (s->length == 0) return rec_fail(-2, "%s: length must be positive", fn);
+    if (s->length == 1 && !s->marks) {
+        if ((int64_t)s->batch * s->channels > (int64_t)0x7fffffff * 32) return rec_fail(-2, "%s: sizes too large", fn);
+        Plan none;
+        memset(&none, 0, sizeof none);
+        const ScanArgs a = args_of(s, none, nullptr);
+        rec_typed(s->dtype, [&](auto v) {
+            typedef decltype(v) T;
+            if (s->states <= 4)
+                launch_step<T, 1>(s, a, st);
+            else if (s->states <= 8)
+                launch_step<T, 2>(s, a, st);
+            else if (s->states <= 16)
+                launch_step<T, 4>(s, a, st);
+            else
+                launch_step<T, 8>(s, a, st);
+            return 0;
+        });
+        return rec_launched(fn);
+    }
+    const Plan p = plan_of(s, false);
+    rc = check_workspace(fn, p, workspace, workspace_size);
+    if (rc) return rc;
+    const ScanArgs a = args_of(s, p, (uint8_t*)workspace);
+    const int64_t grid = (int64_t)s->batch * p.chunks * p.blocks;
+    if (grid > 0x7fffffff || (int64_t)s->batch * s->length * 2 * p.NS > (int64_t)0x7fffffff * 256)
+        return rec_fail(-2, "%s: sizes too large", fn);
+    rec_typed(s->dtype, [&](auto v) {
+        typedef decltype(v) T;
+        return with_states(p.NS, [&](auto ns) {
+            constexpr int NS = decltype(ns)::value;
+            launch_pack<T, NS>(s, a, st);
+            if (p.chunks > 1) {
+                scan_forward<T, NS, true><<<(unsigned)grid, 64, 0, st>>>(a);
+                scan_join<false><<<(unsigned)(((int64_t)s->batch * NS * s->channels + 255) / 256), 256, 0, st>>>(
+                    a.ends, a.prods, s->state, s->batch, p.chunks, NS, s->channels, s->states);
+            }
+            scan_forward<T, NS, false><<<(unsigned)grid, 64, 0, st>>>(a);
+            return 0;
+        });
+    });
+    return rec_launched(fn);
+}
+
+SDFR_API int32_t sdfr_scan_grad(const SdfrScan* s, const SdfrScanGrad* g, void* workspace, int64_t workspace_size,
+                                void* stream) {
+    const char* fn = "sdfr_scan_grad";
+    int32_t rc = check_scan(fn, s);
+    if (rc) return rc;
+    if (!g) return rec_fail(-1, "%s: null gradient descriptor", fn);
+    if (s->batch == 0 || s->length == 0) return rec_fail(-2, "%s: nothing to differentiate", fn);
+    if (!s->marks || !g->dout || !g->dx || !g->ddt || !g->dA || !g->dB || !g->dC || (s->z && !g->dz))
+        return rec_fail(-1, "%s: null pointer argument", fn);
+    const Plan p = plan_of(s, true);
+    rc = check_workspace(fn, p, workspace, workspace_size);
+    if (rc) return rc;
+    hipStream_t st = (hipStream_t)stream;
+    uint8_t* ws = (uint8_t*)workspace;
+    const ScanArgs a = args_of(s, p, ws);
+    GradArgs ga;
+    ga.dout = {g->dout, g->dout_b, g->dout_t};
+    ga.dstate_out = g->dstate_out;
+    ga.dx = g->dx;
+    ga.ddt = g->ddt;
+    ga.dz = g->dz;
+    ga.dstate = g->dstate;
+    ga.bc_part = (float*)(ws + p.part);
+    ga.sums = (float*)(ws + p.sums);
+    ga.ends = a.ends;
+    const int64_t grid = (int64_t)s->batch * p.chunks * p.blocks, rows = (int64_t)s->batch * s->length;
+    if (grid > 0x7fffffff || rows * 2 * p.NS > (int64_t)0x7fffffff * 256)
+        return rec_fail(-2, "%s: sizes too large", fn);
+    rec_typed(s->dtype, [&](auto v) {
+        typedef decltype(v) T;
+        return with_states(p.NS, [&](auto ns) {
+            constexpr int NS = decltype(ns)::value;
+            launch_pack<T, NS>(s, a, st);
+            if (p.chunks > 1) {
+                scan_backward_ends<T, NS><<<(unsigned)grid, 64, 0, st>>>(a, ga);
+                scan_join<true><<<(unsigned)(((int64_t)s->batch * NS * s->channels + 255) / 256), 256, 0, st>>>(
+                    a.ends, a.prods, g->dstate_out, s->batch, p.chunks, NS, s->channels, s->states);
+            }
+            scan_backward<T, NS><<<(unsigned)grid, 64, 0, st>>>(a, ga);
+            bc_sums<T, NS><<<(unsigned)((rows * 2 * NS + 255) / 256), 256, 0, st>>>(
+                ga.bc_part, (T*)g->dB, (T*)g->dC, rows, p.blocks, s->states);
+            column_sums<<<(unsigned)(((int64_t)(NS + 2) * s->channels + 63) / 64), dim3(64, 16), 0, st>>>(
+                ga.sums, g->dA, g->dskip, g->ddt_bias, (int64_t)s->batch * p.chunks, NS, s->channels, s->states);
+            return 0;
+        });
+    });
+    return rec_launched(fn);
+}
+
+}  // extern "C"

@@ -18,7 +18,7 @@ import torch  # noqa: F401  (load torch's HIP runtime first, see above)
 PKG_ROOT = Path(__file__).resolve().parents[1]
 LIB_PATH = PKG_ROOT / "lib" / "libsdfr.so"
 
-ABI_VERSION = 14
+ABI_VERSION = 15
 NOALLOC_SCRATCH_BYTES = 24 << 20   # SDFR_NOALLOC_SCRATCH_BYTES
 
 # element types (SDFR_* in sdfr.h)
@@ -37,7 +37,10 @@ EXPORTS = ("sdfr_abi_version", "sdfr_last_error", "sdfr_grid_create", "sdfr_grid
            "sdfr_grid_read",
            "sdfr_edt_workspace_bytes",
            "sdfr_edt", "sdfr_edt_last_error", "sdfr_goal_workspace_bytes", "sdfr_goal_bake",
-           "sdfr_goal_sample", "sdfr_goal_yaw", "sdfr_goal_last_error")
+           "sdfr_goal_sample", "sdfr_goal_yaw", "sdfr_goal_last_error",
+           "sdfr_conv", "sdfr_conv_grad_workspace_bytes", "sdfr_conv_grad",
+           "sdfr_scan_workspace_bytes", "sdfr_scan_marks_bytes", "sdfr_scan", "sdfr_scan_grad",
+           "sdfr_draw", "sdfr_clip_workspace_bytes", "sdfr_clip", "sdfr_recurrent_last_error")
 
 
 class GridDesc(ctypes.Structure):
@@ -72,6 +75,41 @@ class GoalInfo(ctypes.Structure):
     _fields_ = [("reach_max", ctypes.c_float), ("sentinel", ctypes.c_float),
                 ("quant", ctypes.c_float), ("sweeps", ctypes.c_int32),
                 ("n_seed", ctypes.c_int64), ("tile_visits", ctypes.c_int64)]
+
+
+def _fields(text: str):
+    """ctypes fields from "name:kind" words; p pointer, q int64, i int32, f float."""
+    kinds = {"p": ctypes.c_void_p, "q": ctypes.c_int64, "i": ctypes.c_int32, "f": ctypes.c_float}
+    return [(n, kinds[k]) for n, k in (w.split(":") for w in text.split())]
+
+
+class Conv(ctypes.Structure):
+    _fields_ = _fields("x:p x_b:q x_t:q weight:p bias:p resets:p resets_b:q resets_t:q state:p "
+                       "y:p y_b:q y_t:q state_out:p length:q batch:i channels:i width:i dtype:i silu:i")
+
+
+class ConvGrad(ctypes.Structure):
+    _fields_ = _fields("dy:p dy_b:q dy_t:q dstate_out:p dx:p dstate:p dweight:p dbias:p")
+
+
+class Scan(ctypes.Structure):
+    _fields_ = _fields("x:p x_b:q x_t:q dt:p dt_b:q dt_t:q z:p z_b:q z_t:q B:p B_b:q B_t:q C:p C_b:q C_t:q "
+                       "A:p skip:p dt_bias:p resets:p resets_b:q resets_t:q state:p state_out:p marks:p "
+                       "y:p y_b:q y_t:q length:q batch:i channels:i states:i dtype:i softplus:i")
+
+
+class ScanGrad(ctypes.Structure):
+    _fields_ = _fields("dout:p dout_b:q dout_t:q dstate_out:p dx:p ddt:p dz:p dB:p dC:p dA:p dskip:p "
+                       "ddt_bias:p dstate:p")
+
+
+class Draw(ctypes.Structure):
+    _fields_ = _fields("logits:p logits_row:q mask:p mask_row:q uniform:p temperature:p top_k:p top_p:p "
+                       "min_p:p temperature1:f top_k1:i top_p1:f min_p1:f token:p logp:p rows:i vocab:i dtype:i")
+
+
+class Tensor(ctypes.Structure):
+    _fields_ = _fields("in_:p out:p size:q dtype:i")
 
 
 class SdfrError(RuntimeError):
@@ -147,6 +185,28 @@ def load(path: Path | str | None = None):
     lib.sdfr_goal_yaw.argtypes = lib.sdfr_goal_sample.argtypes
     lib.sdfr_goal_last_error.restype = ctypes.c_char_p
     lib.sdfr_goal_last_error.argtypes = []
+    lib.sdfr_conv.restype = i32
+    lib.sdfr_conv.argtypes = [ctypes.POINTER(Conv), vp]
+    lib.sdfr_conv_grad_workspace_bytes.restype = i64
+    lib.sdfr_conv_grad_workspace_bytes.argtypes = [ctypes.POINTER(Conv)]
+    lib.sdfr_conv_grad.restype = i32
+    lib.sdfr_conv_grad.argtypes = [ctypes.POINTER(Conv), ctypes.POINTER(ConvGrad), vp, i64, vp]
+    lib.sdfr_scan_workspace_bytes.restype = i64
+    lib.sdfr_scan_workspace_bytes.argtypes = [ctypes.POINTER(Scan), i32]
+    lib.sdfr_scan_marks_bytes.restype = i64
+    lib.sdfr_scan_marks_bytes.argtypes = [ctypes.POINTER(Scan)]
+    lib.sdfr_scan.restype = i32
+    lib.sdfr_scan.argtypes = [ctypes.POINTER(Scan), vp, i64, vp]
+    lib.sdfr_scan_grad.restype = i32
+    lib.sdfr_scan_grad.argtypes = [ctypes.POINTER(Scan), ctypes.POINTER(ScanGrad), vp, i64, vp]
+    lib.sdfr_draw.restype = i32
+    lib.sdfr_draw.argtypes = [ctypes.POINTER(Draw), vp]
+    lib.sdfr_clip_workspace_bytes.restype = i64
+    lib.sdfr_clip_workspace_bytes.argtypes = [ctypes.POINTER(Tensor), i32]
+    lib.sdfr_clip.restype = i32
+    lib.sdfr_clip.argtypes = [ctypes.POINTER(Tensor), i32, ctypes.c_double, ctypes.c_double, vp, vp, i64, vp]
+    lib.sdfr_recurrent_last_error.restype = ctypes.c_char_p
+    lib.sdfr_recurrent_last_error.argtypes = []
     got = lib.sdfr_abi_version()
     if got != ABI_VERSION:
         raise SdfrError(f"{p} reports ABI {got}, this binding mirrors ABI {ABI_VERSION}: "
