@@ -30,7 +30,8 @@ def test_structs_match_the_header_layout(tmp_path):
     for line in got.splitlines():
         cname, field, value = line.split()
         cls = structs[cname]
-        assert int(value) == (ctypes.sizeof(cls) if field == "size" else getattr(cls, field).offset), line
+        at = getattr(cls, field + "_" if field == "in" else field, None)
+        assert int(value) == (ctypes.sizeof(cls) if field == "sizeof" else at.offset), line
 
 
 def _conv(**kw):
