@@ -56,11 +56,32 @@ __device__ inline u64 share(uint32_t part, u64 total, bool up) {
     return (u64)part * (total >> 32) * 256 + ((low + (up ? 0xffffffu : 0u)) >> 24);
 }
 
-__device__ inline u64 wave_sum(u64 v) {
-#pragma unroll
-    for (int m = 32; m > 0; m /= 2) v += __shfl_xor(v, m);
+// Sums over a wave by cross-lane moves: eight lanes' neighbours, then rows of
+// 16, then the halves; the total is in lane 63.
+template <int CTRL, int ROWS>
+__device__ inline u64 moved(u64 v) {
+    const int lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, CTRL, ROWS, 0xf, false);
+    const int hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(v >> 32), CTRL, ROWS, 0xf, false);
+    return (u64)(uint32_t)hi << 32 | (uint32_t)lo;
+}
+
+// The running sum over the lanes up to and with this one.
+__device__ inline u64 wave_scan(u64 v) {
+    v += moved<0x111, 0xf>(v);   // from 1, 2, 4, 8 lanes below in the row of 16
+    v += moved<0x112, 0xf>(v);
+    v += moved<0x114, 0xf>(v);
+    v += moved<0x118, 0xf>(v);
+    v += moved<0x142, 0xa>(v);   // lane 15 of rows 0 and 2 into rows 1 and 3
+    v += moved<0x143, 0xc>(v);   // lane 31 into the upper half
     return v;
 }
+
+__device__ inline u64 last_lane(u64 v) {
+    const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)v, 63);
+    const uint32_t hi = __builtin_amdgcn_readlane((int)(uint32_t)(v >> 32), 63);
+    return (u64)hi << 32 | lo;
+}
+__device__ inline u64 wave_sum(u64 v) { return last_lane(wave_scan(v)); }
 
 // A row's settings; threads of a row agree on them.
 struct Settings {
@@ -91,268 +112,582 @@ __device__ inline uint32_t chance_of(float u) {
     return v >= 16777215.0f ? 16777215u : v > 0.0f ? (uint32_t)v : 0u;
 }
 
-// What a row's threads hold of it: lanes take V neighbours, waves whole
-// stretches, so that (wave, turn, lane, neighbour) is the order of indices.
-template <typename T, int THREADS>
+// What a wave holds of a row: lanes take V neighbours, waves whole stretches,
+// so that (wave, turn, lane, neighbour) is the order of indices.
+template <typename T>
 struct Row {
     static constexpr int V = 16 / sizeof(T);
-    static constexpr int WAVES = THREADS / 64;
     const T* p;
     const uint8_t* mask;
-    int vocab, from, to, lane;
+    int vocab;
 
-    __device__ Row(const DrawArgs& a, int row) {
-        p = (const T*)a.logits + row * a.row;
-        mask = a.mask ? a.mask + row * a.mask_row : nullptr;
-        vocab = a.vocab;
-        lane = threadIdx.x & 63;
-        const int turn = 64 * V;
-        const int turns = (vocab + turn - 1) / turn;
-        const int each = (turns + WAVES - 1) / WAVES * turn;
-        const int64_t f = (int64_t)(threadIdx.x / 64) * each;
-        from = f < vocab ? (int)f : vocab;
-        to = vocab - from < each ? vocab : from + each;
-    }
-    // V logits at index i; what is masked or past the end is -inf
-    __device__ void load(int i, float (&x)[V]) const {
+    __device__ Row(const DrawArgs& a, int row)
+        : p((const T*)a.logits + row * a.row), mask(a.mask ? a.mask + row * a.mask_row : nullptr), vocab(a.vocab) {}
+
+    struct Vec {
+        T r[V];
+    };
+    // V logits from index i on; what is masked or past the end is -inf
+    __device__ Vec load(int i) const {
+        Vec v;
         if (i + V <= vocab) {
-            T r[V];
-            __builtin_memcpy(r, p + i, sizeof r);
-#pragma unroll
-            for (int j = 0; j < V; ++j) x[j] = (float)r[j];
+            __builtin_memcpy(v.r, p + i, sizeof v.r);
             if (mask) {
                 uint8_t ok[V];
                 __builtin_memcpy(ok, mask + i, V);
 #pragma unroll
                 for (int j = 0; j < V; ++j)
-                    if (!ok[j]) x[j] = -INFINITY;
+                    if (!ok[j]) v.r[j] = (T)-INFINITY;
             }
         } else {
 #pragma unroll
-            for (int j = 0; j < V; ++j) x[j] = i + j < vocab && (!mask || mask[i + j]) ? (float)p[i + j] : -INFINITY;
+            for (int j = 0; j < V; ++j) v.r[j] = i + j < vocab && (!mask || mask[i + j]) ? p[i + j] : (T)-INFINITY;
         }
-    }
-    // Calls f(first index, logits) for this lane's vectors, in order, by all lanes of the wave alike.
-    template <class F>
-    __device__ void each(F f) const {
-        for (int i = from; i < to; i += 64 * V) {
-            float x[V];
-            load(i + lane * V, x);
-            f(i + lane * V, x);
-        }
+        return v;
     }
 };
 
-// Sums over the block of one or two numbers a thread.
-template <int THREADS>
-__device__ inline u64 block_sum(u64 v, u64* lds) {
-    v = wave_sum(v);
-    if constexpr (THREADS == 64) return v;
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) lds[threadIdx.x / 64] = v;
-    __syncthreads();
-    u64 s = 0;
-#pragma unroll
-    for (int j = 0; j < THREADS / 64; ++j) s += lds[j];
-    return s;
+// The threshold: candidates whose key is above it are kept, and the first
+// `take` of those that equal it.
+struct Cut {
+    uint32_t key;
+    u64 take;
+};
+
+__device__ inline void answer(const DrawArgs& a, int row, int64_t token, float logp) {
+    a.token[row] = token;
+    a.logp[row] = logp;
 }
 
-template <typename T, int THREADS>
-__global__ __launch_bounds__(THREADS) void draw_rows(DrawArgs a) {
-    constexpr int WAVES = THREADS / 64;
-    __shared__ u64 lds[WAVES + 1];
-    __shared__ u64 sums[WAVES];
-    __shared__ int ties[WAVES];
-    const int row = blockIdx.x;
-    const int wave = threadIdx.x / 64;
+__device__ inline float logp_of(float z, u64 total) { return z - logf((float)total * 9.094947017729282e-13f); }
+
+// The lowest bit that tells two keys of a type apart: below it a positive
+// number's are all 0 and a negative one's all 1.
+template <typename T> constexpr int kLowBit = 0;
+template <> constexpr int kLowBit<_Float16> = 13;
+template <> constexpr int kLowBit<__bf16> = 16;
+template <typename T>
+__device__ inline uint32_t whole_key(uint32_t k) {
+    return k & 0x80000000u ? k : k | ((1u << kLowBit<T>) - 1);
+}
+
+// ---- small vocabularies: a wave a row ------------------------------------------
+// All of a row's weights are in registers; the thresholds are searched bit by
+// bit, counts by ballots.
+template <typename T, int E>   // E: candidates a lane
+__global__ __launch_bounds__(256) void draw_small(DrawArgs a) {
+    constexpr int V = Row<T>::V, TURNS = E / V;
+    const int row = blockIdx.x * 4 + threadIdx.x / 64, lane = threadIdx.x & 63;
+    if (row >= a.rows) return;
     const Settings s = settings_of(a, row);
-    const Row<T, THREADS> r(a, row);
-    constexpr int V = Row<T, THREADS>::V;
+    const Row<T> r(a, row);
+    float x[E];
+    float m = -INFINITY;
+    bool bad = false;
+#pragma unroll
+    for (int q = 0; q < TURNS; ++q) {
+        const auto v = r.load((q * 64 + lane) * V);
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            x[q * V + j] = (float)v.r[j];
+            m = fmaxf(m, x[q * V + j]);
+            bad |= x[q * V + j] != x[q * V + j];
+        }
+    }
+#pragma unroll
+    for (int d = 32; d > 0; d /= 2) m = fmaxf(m, __shfl_xor(m, d));
+    if (__ballot(bad)) return answer(a, row, -1, NAN);   // every lane writes the same
+    if (m == -INFINITY) return answer(a, row, -1, 0.0f);
+    const float inv_t = s.greedy ? 1.0f : s.inv_t;
+    uint32_t key[E];
+    u64 w[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        key[e] = key_of(x[e]);
+        w[e] = weight(expf(z_of(x[e], m, inv_t)));
+    }
+    Cut cut = {0, ~0ull};
+    if (s.greedy || s.k == 1) {
+        cut = {key_of(m), 1};
+    } else {
+        auto count = [&](uint32_t t) {   // of keys that reach t; what lies past the end does not
+            int n = 0;
+#pragma unroll
+            for (int e = 0; e < E; ++e) n += __popcll(__ballot(key[e] >= t));
+            return n;
+        };
+        if (s.k > 0) {
+            uint32_t k = 0;
+            for (int bit = 31; bit >= kLowBit<T>; --bit)
+                if (count(k | 1u << bit) >= s.k) k |= 1u << bit;
+            k = whole_key<T>(k);
+            cut = {k, (u64)(s.k - (k == 0xffffffffu ? 0 : count(k + 1)))};
+        }
+        if (s.cut) {
+            const u64 tie = s.k > 0 ? weight(expf(z_of(of_key(cut.key), m, inv_t))) : 0;
+            auto mass = [&](uint32_t t) {   // of the kept ones that reach t
+                u64 v = 0;
+                int ties = 0;
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    v += key[e] >= t && key[e] > cut.key ? w[e] : 0;
+                    if (s.k > 0) ties += __popcll(__ballot(key[e] >= t && key[e] == cut.key));
+                }
+                return wave_sum(v) + ((u64)ties < cut.take ? (u64)ties : cut.take) * tie;
+            };
+            u64 bound = share(s.p24, mass(0), true);
+            if (bound == 0) bound = 1;
+            uint32_t k = 0;
+            for (int bit = 31; bit >= kLowBit<T>; --bit)
+                if (mass(k | 1u << bit) >= bound) k |= 1u << bit;
+            k = whole_key<T>(k);
+            const u64 above = k == 0xffffffffu ? 0 : mass(k + 1);
+            const u64 each = weight(expf(z_of(of_key(k), m, inv_t)));   // not 0: the bound is reached here
+            u64 n = (bound - above + each - 1) / each;
+            if (s.k > 0 && k == cut.key && n > cut.take) n = cut.take;
+            cut = {k, n};
+        }
+    }
+    // what is kept, in the order of indices: first the ties' ranks, then the running sums
+    u64 total = 0, left = cut.take, before[TURNS], upto[TURNS];
+#pragma unroll
+    for (int q = 0; q < TURNS; ++q) {
+        int ties = 0, rank = 0, all = 0;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const uint64_t b = __ballot(key[q * V + j] == cut.key);
+            rank += __popcll(b & ((1ull << lane) - 1));
+            all += __popcll(b);
+        }
+        u64 sum = 0;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const int e = q * V + j;
+            bool keep = key[e] > cut.key;
+            if (key[e] == cut.key) keep = (u64)(rank + ties++) < left;
+            if (!keep || !(expf(z_of(x[e], m, inv_t)) >= s.min_p)) w[e] = 0;
+            sum += w[e];
+        }
+        left -= (u64)all < left ? (u64)all : left;
+        upto[q] = wave_scan(sum);
+        const u64 turn = last_lane(upto[q]);
+        upto[q] += total;
+        before[q] = upto[q] - sum;
+        total += turn;
+    }
+    const u64 target = share(chance_of(a.uniform[row]), total, false);
+#pragma unroll
+    for (int q = 0; q < TURNS; ++q) {
+        if (target < before[q] || target >= upto[q]) continue;
+        u64 run = before[q];
+        int at = 0;
+        float xt = 0.0f;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            if (target >= run && target < run + w[q * V + j]) {
+                at = j;
+                xt = x[q * V + j];
+            }
+            run += w[q * V + j];
+        }
+        answer(a, row, (q * 64 + lane) * V + at, s.greedy ? 0.0f : logp_of(z_of(xt, m, inv_t), total));
+    }
+}
+
+// ---- large vocabularies: a workgroup a row ----------------------------------------
+// The thresholds come from histograms in LDS: candidates fall into bins by
+// their distance from the largest, a scan over the bins from the top finds the
+// one in which the count or the mass passes its bound, and within that bin the
+// keys are ranked against each other (or, where there are too many of them,
+// fall into bins by key until one bin holds a single key or few enough).
+// Bins first take the nearest kNear only, where the answer nearly always lies,
+// so most candidates cost no LDS operation; beyond kFar weights are zero, and
+// a threshold there is none. Sums are of integers, so the order in which the
+// LDS takes them does not matter.
+//
+// A top-p threshold after a top-k one needs no list of what top-k left: its
+// bound is a share of that mass, which is reached at or above the top-k key,
+// and among the ties there no later than the last one taken.
+constexpr int kBins = 2048, kList = 256;
+constexpr float kNear = 8.0f, kFar = 28.0f;
+
+template <int THREADS>
+struct Shared {
+    u64 mass[kBins];
+    uint32_t count[kBins];
+    uint32_t list[kList];
+    u64 part[THREADS / 64], part2[THREADS / 64];
+    u64 turn[THREADS];            // kept mass of each turn of each wave
+    int ties[THREADS];            // and its candidates at the threshold
+    uint32_t fill, lo, hi, bin, key, at;
+    u64 above_count, above_mass, take, before, mass_kept;
+};
+
+template <typename T, int THREADS>
+struct Block {
+    static constexpr int V = Row<T>::V, WAVES = THREADS / 64, N = kBins / THREADS;
+    const Row<T> r;
+    Shared<THREADS>& sh;
+    const Settings& s;
+    const int lane, wave;
+    int turns;              // of each wave
+    float m, inv_t;
+    int have = -1;          // the range whose bins are in LDS
+    u64 low = 0;            // this thread's mass beyond kNear
+
+    __device__ __forceinline__ Block(const DrawArgs& a, int row, Shared<THREADS>& shared, const Settings& settings)
+        : r(a, row), sh(shared), s(settings), lane(threadIdx.x & 63), wave(threadIdx.x / 64) {
+        const int all = (a.vocab + 64 * V - 1) / (64 * V);
+        turns = (all + WAVES - 1) / WAVES;
+    }
+    __device__ __forceinline__ int index(int turn) const { return ((wave * turns + turn) * 64 + lane) * V; }
+    // Calls f(turn, logits) for the wave's turns in order, with all lanes; the next three turns' loads are in flight.
+    template <class F>
+    __device__ __forceinline__ void each(F f) const {
+        typename Row<T>::Vec ahead[3] = {r.load(index(0)), r.load(index(1)), r.load(index(2))};
+#pragma unroll 1
+        for (int t = 0; t < turns; ++t) {
+            float x[V];
+#pragma unroll
+            for (int j = 0; j < V; ++j) x[j] = (float)ahead[0].r[j];
+            ahead[0] = ahead[1];
+            ahead[1] = ahead[2];
+            ahead[2] = r.load(index(t + 3));
+            f(t, x);
+        }
+    }
+    __device__ __forceinline__ float z(float x) const { return z_of(x, m, inv_t); }
+    __device__ __forceinline__ u64 w(float x) const { return weight(expf(z(x))); }
+
+    __device__ __forceinline__ u64 sum(u64 v) const {
+        v = wave_sum(v);
+        __syncthreads();
+        if (lane == 0) sh.part[wave] = v;
+        __syncthreads();
+        u64 t = 0;
+#pragma unroll
+        for (int j = 0; j < WAVES; ++j) t += sh.part[j];
+        return t;
+    }
+    // The sum over the threads before this one, and over all.
+    __device__ __forceinline__ u64 scan(u64 v, u64* all) const {
+        const u64 u = wave_scan(v);
+        const u64 t = last_lane(u);
+        __syncthreads();
+        if (lane == 0) sh.part[wave] = t;
+        __syncthreads();
+        u64 before = u - v, sum = 0;
+#pragma unroll
+        for (int j = 0; j < WAVES; ++j) {
+            if (j < wave) before += sh.part[j];
+            sum += sh.part[j];
+        }
+        *all = sum;
+        return before;
+    }
+
+    __device__ __forceinline__ void clear() {
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < N; ++i) sh.mass[threadIdx.x + i * THREADS] = 0, sh.count[threadIdx.x + i * THREADS] = 0;
+        if (threadIdx.x == 0) sh.fill = 0, sh.lo = 0xffffffffu, sh.hi = 0;
+        __syncthreads();
+    }
+    // Distances (from, to] of a range, and its bins; -1: outside.
+    __device__ __forceinline__ static int bin_of(float z, int range) {
+        const float from = range ? kNear : 0.0f, to = range ? kFar : kNear;
+        if (!(z > -to) || (range && z > -from)) return -1;
+        const int b = (int)((-z - from) * (kBins / (to - from)));
+        return b < kBins ? b : kBins - 1;
+    }
+    // Fills the bins with a range. With top-p, masses too, and the first time
+    // the mass of what lies further off.
+    __device__ __forceinline__ void fill(int range, bool want_low) {
+        clear();
+        u64 l = 0;
+        each([&](int, float(&x)[V]) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const float zj = z(x[j]);
+                const int b = bin_of(zj, range);
+                if (b >= 0) {
+                    atomicAdd(&sh.count[b], 1u);
+                    if (s.cut) atomicAdd(&sh.mass[b], weight(expf(zj)));
+                } else if (want_low && zj > -kFar) {
+                    l += weight(expf(zj));
+                }
+            }
+        });
+        if (want_low) low = l;
+        have = range;
+        __syncthreads();
+    }
+    __device__ __forceinline__ void totals(u64* c, u64* v) const {
+        u64 tc = 0, tv = 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i) tc += sh.count[threadIdx.x + i * THREADS], tv += sh.mass[threadIdx.x + i * THREADS];
+        *c = sum(tc);
+        *v = sum(tv);
+    }
+    // The first bin at which the running count (or mass) reaches `bound`: into
+    // sh.bin, with what lies in the bins before. False if none does.
+    __device__ __forceinline__ bool find(bool by_mass, u64 bound) {
+        u64 c[N], v[N], cs = 0, vs = 0;
+        __syncthreads();
+        if (threadIdx.x == 0) sh.bin = kBins;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            c[i] = sh.count[threadIdx.x * N + i];
+            v[i] = sh.mass[threadIdx.x * N + i];
+            cs += c[i];
+            vs += v[i];
+        }
+        u64 all;
+        u64 cb = scan(cs, &all), vb = s.cut ? scan(vs, &all) : 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const u64 before = by_mass ? vb : cb, n = by_mass ? v[i] : c[i];
+            if (before < bound && before + n >= bound) {   // one thread's one bin
+                sh.bin = threadIdx.x * N + i;
+                sh.above_count = cb;
+                sh.above_mass = vb;
+            }
+            cb += c[i];
+            vb += v[i];
+        }
+        __syncthreads();
+        return sh.bin < kBins;
+    }
+    // Keys of one bin, between lo and hi, into the list if they fit, and their
+    // lowest and highest.
+    __device__ __forceinline__ void collect(int range, int bin, uint32_t lo, uint32_t hi, uint32_t members) {
+        clear();
+        have = -1;
+        each([&](int, float(&x)[V]) {
+#pragma unroll
+            for (int j = 0; j < V; ++j)
+                if (bin_of(z(x[j]), range) == bin) {
+                    const uint32_t k = key_of(x[j]);
+                    if (k >= lo && k <= hi) {
+                        if (members <= kList) sh.list[atomicAdd(&sh.fill, 1u)] = k;
+                        atomicMin(&sh.lo, k);
+                        atomicMax(&sh.hi, k);
+                    }
+                }
+        });
+        __syncthreads();
+    }
+    // The threshold at which the running count or mass, from the top, reaches
+    // `bound`; `kept`: the mass up to there (with top-p). False where it lies
+    // among weights of zero.
+    __device__ __forceinline__ bool threshold(bool by_mass, u64 bound, Cut* cut, u64* kept) {
+        u64 above_c = 0, above_m = 0;
+        int range = 0;
+        if (have != 0) fill(0, false);
+        if (!find(by_mass, bound)) {
+            totals(&above_c, &above_m);
+            fill(1, false);
+            range = 1;
+            if (!find(by_mass, bound - (by_mass ? above_m : above_c))) return false;
+        }
+        const int bin = (int)sh.bin;
+        uint32_t members = sh.count[bin];
+        above_c += sh.above_count;
+        above_m += sh.above_mass;
+        collect(range, bin, 0, 0xffffffffu, members);
+        uint32_t lo = sh.lo, hi = sh.hi;
+        while (members > kList && lo != hi) {
+            int shift = 0;
+            while ((hi - lo) >> shift >= (uint32_t)kBins) ++shift;
+            clear();
+            each([&](int, float(&x)[V]) {
+#pragma unroll
+                for (int j = 0; j < V; ++j)
+                    if (bin_of(z(x[j]), range) == bin) {
+                        const uint32_t k = key_of(x[j]);
+                        if (k >= lo && k <= hi) {
+                            atomicAdd(&sh.count[(hi - k) >> shift], 1u);
+                            if (s.cut) atomicAdd(&sh.mass[(hi - k) >> shift], w(x[j]));
+                        }
+                    }
+            });
+            find(by_mass, bound - (by_mass ? above_m : above_c));
+            const uint32_t q = sh.bin;   // its keys: hi - k from q << shift on, 1 << shift of them
+            members = sh.count[q];
+            above_c += sh.above_count;
+            above_m += sh.above_mass;
+            const uint32_t top = hi - (q << shift), width = (1u << shift) - 1;
+            collect(range, bin, top - lo < width ? lo : top - width, top, members);
+            lo = sh.lo;
+            hi = sh.hi;
+        }
+        if (lo == hi) {
+            if (threadIdx.x == 0) {
+                const u64 v = w(of_key(lo));
+                sh.key = lo;
+                sh.take = by_mass ? (bound - above_m + v - 1) / v : bound - above_c;
+                sh.mass_kept = above_m + sh.take * v;
+            }
+        } else if (threadIdx.x < members) {
+            const uint32_t k = sh.list[threadIdx.x];
+            u64 c = above_c, v = above_m, ties = 0;
+            for (uint32_t i = 0; i < members; ++i) {
+                const uint32_t o = sh.list[i];
+                ties += o == k;
+                if (o > k) {
+                    c += 1;
+                    if (s.cut) v += w(of_key(o));
+                }
+            }
+            const u64 each_w = s.cut ? w(of_key(k)) : 0;
+            const u64 before = by_mass ? v : c, all = by_mass ? ties * each_w : ties;
+            if (before < bound && before + all >= bound) {   // ties write the same
+                const u64 take = by_mass ? (bound - before + each_w - 1) / each_w : bound - before;
+                sh.key = k;
+                sh.take = take;
+                sh.mass_kept = v + take * each_w;
+            }
+        }
+        __syncthreads();
+        *cut = {sh.key, sh.take};
+        *kept = sh.mass_kept;
+        return true;
+    }
+};
+
+template <typename T, int THREADS>
+__global__ __launch_bounds__(THREADS) void draw_large(DrawArgs a) {
+    typedef Block<T, THREADS> B;
+    constexpr int V = B::V, WAVES = B::WAVES;
+    __shared__ Shared<THREADS> sh;
+    const int row = blockIdx.x;
+    const Settings s = settings_of(a, row);
+    B b(a, row, sh, s);
 
     // the largest, and whether anything is not a number
     float m = -INFINITY;
     bool bad = false;
-    r.each([&](int, float(&x)[V]) {
+    b.each([&](int, float(&x)[V]) {
 #pragma unroll
         for (int j = 0; j < V; ++j) {
             m = fmaxf(m, x[j]);
             bad |= x[j] != x[j];
         }
     });
-    uint32_t top = key_of(m);
 #pragma unroll
-    for (int k = 32; k > 0; k /= 2) {
-        const uint32_t o = __shfl_xor(top, k);
-        top = o > top ? o : top;
-    }
+    for (int d = 32; d > 0; d /= 2) m = fmaxf(m, __shfl_xor(m, d));
     const bool any_bad = __ballot(bad) != 0;
-    if (WAVES > 1) {
-        if ((threadIdx.x & 63) == 0) lds[wave] = (u64)any_bad << 32 | top;
-        __syncthreads();
-        bad = false;
-        for (int j = 0; j < WAVES; ++j) {
-            bad |= lds[j] >> 32 != 0;
-            top = (uint32_t)lds[j] > top ? (uint32_t)lds[j] : top;
-        }
-        __syncthreads();
-    } else {
-        bad = any_bad;
+    if (b.lane == 0) sh.part[b.wave] = (u64)any_bad << 32 | __float_as_uint(m);
+    __syncthreads();
+    bad = false;
+    for (int j = 0; j < WAVES; ++j) {
+        bad |= sh.part[j] >> 32 != 0;
+        m = fmaxf(m, __uint_as_float((uint32_t)sh.part[j]));
     }
-    m = of_key(top);
     if (bad || m == -INFINITY) {   // nothing to draw from: no number among them, or nothing legal
-        if (threadIdx.x == 0) {
-            a.token[row] = -1;
-            a.logp[row] = bad ? NAN : 0.0f;
-        }
+        if (threadIdx.x == 0) answer(a, row, -1, bad ? NAN : 0.0f);
         return;
     }
-    const float inv_t = s.greedy ? 1.0f : s.inv_t;
+    b.m = m;
+    b.inv_t = s.greedy ? 1.0f : s.inv_t;
 
-    // the threshold: candidates above `key` are kept, and the first `take` that equal it
-    uint32_t key = 0;
-    u64 take = ~0ull;
+    Cut cut = {0, ~0ull};
     if (s.greedy || s.k == 1) {
-        key = top;
-        take = 1;
+        cut = {key_of(m), 1};
     } else {
-        u64 limit = ~0ull;   // of those at the top-k threshold
-        uint32_t kkey = 0;
-        if (s.k > 0) {       // the largest key that at least k candidates reach
-            for (int bit = 31; bit >= 0; --bit) {
-                const uint32_t t = kkey | 1u << bit;
-                u64 n = 0;
-                r.each([&](int i, float(&x)[V]) {
-#pragma unroll
-                    for (int j = 0; j < V; ++j) n += i + j < a.vocab && key_of(x[j]) >= t;
-                });
-                if (block_sum<THREADS>(n, lds) >= (u64)s.k) kkey = t;
-            }
-            u64 above = 0;
-            r.each([&](int, float(&x)[V]) {
-#pragma unroll
-                for (int j = 0; j < V; ++j) above += key_of(x[j]) > kkey;
-            });
-            limit = s.k - block_sum<THREADS>(above, lds);
-            key = kkey;
-            take = limit;
-        }
-        if (s.cut) {
-            // mass of the kept ones that reach t, ties at the top-k threshold counted as far as they are kept
-            auto mass = [&](uint32_t t) {
-                u64 w = 0, eq = 0;
-                r.each([&](int, float(&x)[V]) {
-#pragma unroll
-                    for (int j = 0; j < V; ++j) {
-                        const uint32_t k = key_of(x[j]);
-                        if (k >= t && (k > kkey || s.k == 0)) w += weight(expf(z_of(x[j], m, inv_t)));
-                        eq += s.k > 0 && k >= t && k == kkey;
-                    }
-                });
-                w = block_sum<THREADS>(w, lds);
-                if (s.k > 0) {
-                    eq = block_sum<THREADS>(eq, lds);
-                    w += (eq < limit ? eq : limit) * weight(expf(z_of(of_key(kkey), m, inv_t)));
+        u64 kept = 0;
+        bool of_k = false;
+#pragma unroll 1
+        for (int by_mass = s.k > 0 ? 0 : 1; by_mass < (s.cut ? 2 : 1); ++by_mass) {
+            u64 bound = (u64)s.k;
+            if (by_mass) {
+                if (!of_k) {   // a share of all there is
+                    b.fill(0, true);
+                    u64 c, v;
+                    b.totals(&c, &v);
+                    kept = v + b.sum(b.low);
                 }
-                return w;
-            };
-            u64 bound = share(s.p24, mass(0), true);
-            if (bound == 0) bound = 1;
-            uint32_t pkey = 0;   // the largest key whose mass reaches the bound
-            for (int bit = 31; bit >= 0; --bit) {
-                const uint32_t t = pkey | 1u << bit;
-                if (mass(t) >= bound) pkey = t;
+                bound = share(s.p24, kept, true);
+                if (bound == 0) bound = 1;
             }
-            const u64 above = pkey == 0xffffffffu ? 0 : mass(pkey + 1);
-            const u64 each = weight(expf(z_of(of_key(pkey), m, inv_t)));   // not 0: the bound is reached here
-            u64 n = (bound - above + each - 1) / each;
-            if (pkey == kkey && s.k > 0 && n > limit) n = limit;
-            key = pkey;
-            take = n;
+            of_k = b.threshold(by_mass != 0, bound, &cut, &kept);
         }
     }
 
-    // each wave's kept mass and ties
-    u64 w = 0;
-    int eq = 0;
-    r.each([&](int, float(&x)[V]) {
+    // each turn's kept mass, and its candidates at the threshold
+    sh.turn[threadIdx.x] = 0;
+    sh.ties[threadIdx.x] = 0;
+    __syncthreads();
+    b.each([&](int t, float(&x)[V]) {
+        u64 sum = 0;
+        int eq = 0;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
             const uint32_t k = key_of(x[j]);
-            const float e = expf(z_of(x[j], m, inv_t));
-            if (k > key && e >= s.min_p) w += weight(e);
-            eq += k == key;
+            if (k > cut.key) {
+                const float e = expf(b.z(x[j]));
+                if (e >= s.min_p) sum += weight(e);
+            }
+            eq += __popcll(__ballot(k == cut.key));
+        }
+        sum = __ballot(sum != 0) ? wave_sum(sum) : 0;
+        if (b.lane == 0) {
+            sh.turn[b.wave * b.turns + t] = sum;
+            sh.ties[b.wave * b.turns + t] = eq;
         }
     });
-    w = wave_sum(w);
-    eq = (int)wave_sum((u64)eq);
-    const float tie_e = expf(z_of(of_key(key), m, inv_t));
+    const float tie_e = expf(b.z(of_key(cut.key)));
     const u64 tie = tie_e >= s.min_p ? weight(tie_e) : 0;
-    if ((threadIdx.x & 63) == 0) {
-        sums[wave] = w;
-        ties[wave] = eq;
+    __syncthreads();
+    const u64 eq = sh.ties[threadIdx.x];
+    u64 total;
+    const u64 ties_before = b.scan(eq, &total);
+    u64 allowed = cut.take > ties_before ? cut.take - ties_before : 0;
+    const u64 mine = sh.turn[threadIdx.x] + (eq < allowed ? eq : allowed) * tie;
+    const u64 before = b.scan(mine, &total);
+    u64 target = share(chance_of(a.uniform[row]), total, false);
+    if (before <= target && target < before + mine) {   // one thread
+        sh.at = threadIdx.x;
+        sh.before = before;
+        sh.take = allowed;
     }
     __syncthreads();
-    u64 total = 0, before = 0, left = take, allowed = 0;
-    for (int j = 0; j < WAVES; ++j) {
-        const u64 n = (u64)ties[j] < left ? (u64)ties[j] : left;
-        if (j == wave) before = total, allowed = left;
-        total += sums[j] + n * tie;
-        left -= n;
+    if (b.wave != 0) return;
+    // the turn that holds it, candidate by candidate
+    const int i = ((int)sh.at * 64 + b.lane) * V;
+    target -= sh.before;
+    allowed = sh.take;
+    const auto raw = b.r.load(i);
+    float x[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) x[j] = (float)raw.r[j];
+    u64 w[V], sum = 0;
+    int rank = 0, own = 0;
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+        rank += __popcll(__ballot(key_of(x[j]) == cut.key) & ((1ull << b.lane) - 1));
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        const uint32_t k = key_of(x[j]);
+        const float e = expf(b.z(x[j]));
+        bool keep = k > cut.key;
+        if (k == cut.key) keep = (u64)(rank + own++) < allowed;
+        w[j] = keep && e >= s.min_p ? weight(e) : 0;
+        sum += w[j];
     }
-    u64 target = share(chance_of(a.uniform[row]), total, false);
-    const u64 mine = w + ((u64)eq < allowed ? (u64)eq : allowed) * tie;
-    if (target < before || target >= before + mine) return;
-    // the wave that holds it walks its stretch
-    target -= before;
-    for (int i = r.from; i < r.to; i += 64 * V) {
-        float x[V];
-        u64 run[V], lane_sum = 0;
-        r.load(i + r.lane * V, x);
-        int lane_ties = 0;
+    u64 run = wave_scan(sum) - sum;
+    if (target < run || target >= run + sum) return;
+    int at = 0;
+    float xt = 0.0f;
 #pragma unroll
-        for (int j = 0; j < V; ++j) lane_ties += key_of(x[j]) == key;
-        int ties_before = lane_ties;   // inclusive scan over the lanes
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) {
-            const int o = __shfl_up(ties_before, d);
-            if (r.lane >= d) ties_before += o;
+    for (int j = 0; j < V; ++j) {
+        if (target >= run && target < run + w[j]) {
+            at = j;
+            xt = x[j];
         }
-        const int turn_ties = __shfl(ties_before, 63);
-        int rank = ties_before - lane_ties;
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-            const uint32_t k = key_of(x[j]);
-            const float e = expf(z_of(x[j], m, inv_t));
-            bool keep = k > key;
-            if (k == key) keep = (u64)rank++ < allowed;
-            if (keep && e >= s.min_p) lane_sum += weight(e);
-            run[j] = lane_sum;
-        }
-        u64 upto = lane_sum;
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) {
-            const u64 o = __shfl_up(upto, d);
-            if (r.lane >= d) upto += o;
-        }
-        const u64 turn_sum = __shfl(upto, 63);
-        if (target < turn_sum) {
-            const u64 lo = upto - lane_sum;
-            if (target >= lo && target < upto) {
-                int j = 0;
-                while (run[j] + lo <= target) ++j;
-                a.token[row] = i + r.lane * V + j;
-                float xj = x[0];
-#pragma unroll
-                for (int q = 1; q < V; ++q)
-                    if (q == j) xj = x[q];
-                a.logp[row] = s.greedy ? 0.0f
-                                       : z_of(xj, m, inv_t) - logf((float)total * 9.094947017729282e-13f);
-            }
-            return;
-        }
-        target -= turn_sum;
-        allowed -= (u64)turn_ties < allowed ? (u64)turn_ties : allowed;
+        run += w[j];
     }
+    answer(a, row, i + at, s.greedy ? 0.0f : logp_of(b.z(xt), total));
 }
 
 }  // namespace
@@ -390,12 +725,15 @@ SDFR_API int32_t sdfr_draw(const SdfrDraw* s, void* stream) {
     a.vocab = s->vocab;
     rec_typed(s->dtype, [&](auto v) {
         typedef decltype(v) T;
-        if (s->vocab <= 1024)
-            draw_rows<T, 64><<<s->rows, 64, 0, st>>>(a);
+        const unsigned small = (unsigned)((s->rows + 3) / 4);
+        if (s->vocab <= 512)
+            draw_small<T, 8><<<small, 256, 0, st>>>(a);
+        else if (s->vocab <= 1024)
+            draw_small<T, 16><<<small, 256, 0, st>>>(a);
         else if (s->vocab <= 8192)
-            draw_rows<T, 256><<<s->rows, 256, 0, st>>>(a);
+            draw_large<T, 256><<<s->rows, 256, 0, st>>>(a);
         else
-            draw_rows<T, 1024><<<s->rows, 1024, 0, st>>>(a);
+            draw_large<T, 1024><<<s->rows, 1024, 0, st>>>(a);
         return 0;
     });
     return rec_launched(fn);
