@@ -124,24 +124,76 @@ struct Row {
     __device__ Row(const DrawArgs& a, int row)
         : p((const T*)a.logits + row * a.row), mask(a.mask ? a.mask + row * a.mask_row : nullptr), vocab(a.vocab) {}
 
+    static constexpr uint32_t kNone = std::is_same<T, float>::value      ? 0xff800000u
+                                      : std::is_same<T, _Float16>::value ? 0xfc00fc00u
+                                                                         : 0xff80ff80u;   // -inf, or two of them
     struct Vec {
-        T r[V];
+        uint32_t u[4];
+        __device__ __forceinline__ float operator[](int j) const {
+            if constexpr (sizeof(T) == 4)
+                return __uint_as_float(u[j]);
+            else if constexpr (std::is_same<T, __bf16>::value)
+                return __uint_as_float(j & 1 ? u[j / 2] & 0xffff0000u : u[j / 2] << 16);
+            else
+                return (float)__builtin_bit_cast(_Float16, (uint16_t)(u[j / 2] >> (j & 1) * 16));
+        }
     };
-    // V logits from index i on; what is masked or past the end is -inf
-    __device__ Vec load(int i) const {
+    // V logits from index i on; what is masked or past the end is -inf. A
+    // vector past the end is read as the row's last whole one and moved down,
+    // so no lane reads element by element (which costs the registers of eight).
+    __device__ __forceinline__ Vec load(int i) const {
+        const int at = i + V <= vocab ? i : vocab - V;
         Vec v;
-        if (i + V <= vocab) {
-            __builtin_memcpy(v.r, p + i, sizeof v.r);
-            if (mask) {
-                uint8_t ok[V];
-                __builtin_memcpy(ok, mask + i, V);
+        __builtin_memcpy(v.u, p + at, sizeof v.u);
+        if (mask) {
+            uint32_t ok[V / 4];
+            __builtin_memcpy(ok, mask + at, V);
 #pragma unroll
-                for (int j = 0; j < V; ++j)
-                    if (!ok[j]) v.r[j] = (T)-INFINITY;
+            for (int j = 0; j < V; ++j) {
+                const bool legal = ok[j / 4] >> (j % 4) * 8 & 0xff;
+                if constexpr (sizeof(T) == 4) {
+                    v.u[j] = legal ? v.u[j] : kNone;
+                } else {
+                    const uint32_t half = j & 1 ? 0xffff0000u : 0xffffu;
+                    v.u[j / 2] = legal ? v.u[j / 2] : (v.u[j / 2] & ~half) | (kNone & half);
+                }
             }
-        } else {
+        }
+        int down = i - at;   // elements
+        if (down > 0) {
+            if constexpr (sizeof(T) == 2) {
+                if (down & 1) {
 #pragma unroll
-            for (int j = 0; j < V; ++j) v.r[j] = i + j < vocab && (!mask || mask[i + j]) ? p[i + j] : (T)-INFINITY;
+                    for (int q = 0; q < 4; ++q) v.u[q] = (q < 3 ? v.u[q + 1] : kNone) << 16 | v.u[q] >> 16;
+                }
+                down >>= 1;
+            }
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                if (down > q) {
+                    v.u[0] = v.u[1];
+                    v.u[1] = v.u[2];
+                    v.u[2] = v.u[3];
+                    v.u[3] = kNone;
+                }
+            }
+        }
+        return v;
+    }
+    // The same of a row that may be shorter than a vector.
+    __device__ __forceinline__ Vec load_short(int i) const {
+        if (vocab >= V) return load(i);
+        Vec v;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) v.u[q] = kNone;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            if (i + j >= vocab || (mask && !mask[i + j])) continue;
+            if constexpr (sizeof(T) == 4)
+                v.u[j] = __builtin_bit_cast(uint32_t, p[i + j]);
+            else
+                v.u[j / 2] = (v.u[j / 2] & (j & 1 ? 0xffffu : 0xffff0000u)) |
+                             (uint32_t)__builtin_bit_cast(uint16_t, p[i + j]) << (j & 1) * 16;
         }
         return v;
     }
@@ -186,10 +238,10 @@ __global__ __launch_bounds__(256) void draw_small(DrawArgs a) {
     bool bad = false;
 #pragma unroll
     for (int q = 0; q < TURNS; ++q) {
-        const auto v = r.load((q * 64 + lane) * V);
+        const auto v = r.load_short((q * 64 + lane) * V);
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            x[q * V + j] = (float)v.r[j];
+            x[q * V + j] = v[j];
             m = fmaxf(m, x[q * V + j]);
             bad |= x[q * V + j] != x[q * V + j];
         }
@@ -323,6 +375,10 @@ struct Shared {
     u64 above_count, above_mass, take, before, mass_kept;
 };
 
+// Keeps the compiler from working on a lane's candidates side by side, which
+// spills registers; the other waves fill the gaps.
+__device__ __forceinline__ void one_by_one() { __builtin_amdgcn_sched_barrier(0); }
+
 template <typename T, int THREADS>
 struct Block {
     static constexpr int V = Row<T>::V, WAVES = THREADS / 64, N = kBins / THREADS;
@@ -340,16 +396,20 @@ struct Block {
         const int all = (a.vocab + 64 * V - 1) / (64 * V);
         turns = (all + WAVES - 1) / WAVES;
     }
-    __device__ __forceinline__ int index(int turn) const { return ((wave * turns + turn) * 64 + lane) * V; }
     // Calls f(turn, logits) for the wave's turns in order, with all lanes; the next three turns' loads are in flight.
     template <class F>
     __device__ __forceinline__ void each(F f) const {
+        // where the lane starts is worked out anew by every pass: kept, it and what follows from it would be held in
+        // registers through all of them
+        int start = (wave * turns * 64 + lane) * V;
+        asm volatile("" : "+v"(start));
+        auto index = [&](int turn) { return start + turn * 64 * V; };
         typename Row<T>::Vec ahead[3] = {r.load(index(0)), r.load(index(1)), r.load(index(2))};
 #pragma unroll 1
         for (int t = 0; t < turns; ++t) {
             float x[V];
 #pragma unroll
-            for (int j = 0; j < V; ++j) x[j] = (float)ahead[0].r[j];
+            for (int j = 0; j < V; ++j) x[j] = ahead[0][j];
             ahead[0] = ahead[1];
             ahead[1] = ahead[2];
             ahead[2] = r.load(index(t + 3));
@@ -365,7 +425,7 @@ struct Block {
         if (lane == 0) sh.part[wave] = v;
         __syncthreads();
         u64 t = 0;
-#pragma unroll
+#pragma unroll 2
         for (int j = 0; j < WAVES; ++j) t += sh.part[j];
         return t;
     }
@@ -377,7 +437,7 @@ struct Block {
         if (lane == 0) sh.part[wave] = t;
         __syncthreads();
         u64 before = u - v, sum = 0;
-#pragma unroll
+#pragma unroll 2
         for (int j = 0; j < WAVES; ++j) {
             if (j < wave) before += sh.part[j];
             sum += sh.part[j];
@@ -408,6 +468,7 @@ struct Block {
         each([&](int, float(&x)[V]) {
 #pragma unroll
             for (int j = 0; j < V; ++j) {
+                one_by_one();
                 const float zj = z(x[j]);
                 const int b = bin_of(zj, range);
                 if (b >= 0) {
@@ -465,7 +526,8 @@ struct Block {
         have = -1;
         each([&](int, float(&x)[V]) {
 #pragma unroll
-            for (int j = 0; j < V; ++j)
+            for (int j = 0; j < V; ++j) {
+                one_by_one();
                 if (bin_of(z(x[j]), range) == bin) {
                     const uint32_t k = key_of(x[j]);
                     if (k >= lo && k <= hi) {
@@ -474,6 +536,7 @@ struct Block {
                         atomicMax(&sh.hi, k);
                     }
                 }
+            }
         });
         __syncthreads();
     }
@@ -502,7 +565,8 @@ struct Block {
             clear();
             each([&](int, float(&x)[V]) {
 #pragma unroll
-                for (int j = 0; j < V; ++j)
+                for (int j = 0; j < V; ++j) {
+                    one_by_one();
                     if (bin_of(z(x[j]), range) == bin) {
                         const uint32_t k = key_of(x[j]);
                         if (k >= lo && k <= hi) {
@@ -510,6 +574,7 @@ struct Block {
                             if (s.cut) atomicAdd(&sh.mass[(hi - k) >> shift], w(x[j]));
                         }
                     }
+                }
             });
             find(by_mass, bound - (by_mass ? above_m : above_c));
             const uint32_t q = sh.bin;   // its keys: hi - k from q << shift on, 1 << shift of them
@@ -531,6 +596,7 @@ struct Block {
         } else if (threadIdx.x < members) {
             const uint32_t k = sh.list[threadIdx.x];
             u64 c = above_c, v = above_m, ties = 0;
+#pragma unroll 2
             for (uint32_t i = 0; i < members; ++i) {
                 const uint32_t o = sh.list[i];
                 ties += o == k;
@@ -623,6 +689,7 @@ __global__ __launch_bounds__(THREADS) void draw_large(DrawArgs a) {
         int eq = 0;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
+            one_by_one();
             const uint32_t k = key_of(x[j]);
             if (k > cut.key) {
                 const float e = expf(b.z(x[j]));
@@ -660,7 +727,7 @@ __global__ __launch_bounds__(THREADS) void draw_large(DrawArgs a) {
     const auto raw = b.r.load(i);
     float x[V];
 #pragma unroll
-    for (int j = 0; j < V; ++j) x[j] = (float)raw.r[j];
+    for (int j = 0; j < V; ++j) x[j] = raw[j];
     u64 w[V], sum = 0;
     int rank = 0, own = 0;
 #pragma unroll
