@@ -83,7 +83,10 @@ __device__ inline uint64_t resets_at(const ScanArgs& a, int b, int64_t t, int64_
 }
 
 struct Place {
-    int b, s, blk, d;
+    int b, s, blk;
+    int base;        // the wave's first channel
+    unsigned lane;   // this lane's, from there on
+    int d;           // base + lane
     bool live;
     int64_t t0, t1;
 };
@@ -95,9 +98,11 @@ __device__ inline Place place_of(const ScanArgs& a) {
     const int64_t r = id / a.blocks;
     p.s = (int)(r % a.chunks);
     p.b = (int)(r / a.chunks);
-    const int d = p.blk * 64 + threadIdx.x;
-    p.live = d < a.channels;
-    p.d = p.live ? d : a.channels - 1;   // lanes past the end repeat the last channel and write nothing
+    p.base = p.blk * 64;
+    const int left = a.channels - p.base;
+    p.live = (int)threadIdx.x < left;
+    p.lane = p.live ? threadIdx.x : left - 1;   // lanes past the end repeat the last channel and write nothing
+    p.d = p.base + p.lane;
     p.t0 = p.s * a.chunk;
     p.t1 = p.t0 + a.chunk < a.length ? p.t0 + a.chunk : a.length;
     return p;
@@ -141,26 +146,32 @@ __global__ __launch_bounds__(64) void scan_forward(ScanArgs a) {
             h[n] = a.state && n < a.N ? a.state[((int64_t)p.b * a.channels + p.d) * a.N + n] : 0.0f;
     }
     const float skip = a.skip ? a.skip[p.d] : 0.0f, bias = a.bias ? a.bias[p.d] : 0.0f;
-    const T* xp = (const T*)a.x.p + p.b * a.x.b + p.d;
-    const T* dp = (const T*)a.dt.p + p.b * a.dt.b + p.d;
     const bool gated = !ENDS && a.z.p;
-    const T* zp = gated ? (const T*)a.z.p + p.b * a.z.b + p.d : xp;
-    T* yp = ENDS ? nullptr : (T*)a.y + p.b * a.y_b + p.d;
-    const uniform_f32 bc = (uniform_f32)(uintptr_t)(a.bc + (int64_t)p.b * a.length * 2 * NS);
+    // rows of the wave's channels: a uniform address and the lane
+    const T* xp = (const T*)a.x.p + p.b * a.x.b + p.t0 * a.x.t + p.base;
+    const T* dp = (const T*)a.dt.p + p.b * a.dt.b + p.t0 * a.dt.t + p.base;
+    const T* zp = gated ? (const T*)a.z.p + p.b * a.z.b + p.t0 * a.z.t + p.base : xp;
+    const int64_t zt = gated ? a.z.t : 0;
+    T* yp = ENDS ? nullptr : (T*)a.y + p.b * a.y_b + p.t0 * a.y_t + p.base;
+    uniform_f32 row = (uniform_f32)(uintptr_t)(a.bc + ((int64_t)p.b * a.length + p.t0) * 2 * NS);
+    float* marks = !ENDS && a.marks ? a.marks + (((int64_t)p.b * ((a.length + kTile<NS> - 1) / kTile<NS>) + p.t0 / kTile<NS>) * NS) *
+                                                    a.channels + p.base
+                                    : nullptr;
     uint64_t starts = 0;
     bool cut = false;
     float sum = 0.0f;
     T xr[TT], dr[TT], zr[TT];
-    auto fetch = [&](int64_t t) {
+    int left = (int)(p.t1 - p.t0);   // steps not yet fetched (a chunk is short, a whole sequence of 2^31 steps too long)
+    auto fetch = [&]() {
 #pragma unroll
         for (int i = 0; i < TT; ++i) {
-            const int64_t k = t + i < p.t1 ? t + i : p.t1 - 1;
-            xr[i] = xp[k * a.x.t];
-            dr[i] = dp[k * a.dt.t];
-            if (gated) zr[i] = zp[k * a.z.t];
+            xr[i] = xp[p.lane];
+            dr[i] = dp[p.lane];
+            if (!ENDS) zr[i] = zp[p.lane];
+            if (--left > 0) xp += a.x.t, dp += a.dt.t, zp += zt;   // past the end the last one again
         }
     };
-    fetch(p.t0);
+    fetch();
     for (int64_t t = p.t0; t < p.t1; t += TT) {
         if (a.resets && ((t - p.t0) & 63) == 0) starts = resets_at(a, p.b, t, p.t1);
         float x[TT], dl[TT], z[TT];
@@ -170,11 +181,10 @@ __global__ __launch_bounds__(64) void scan_forward(ScanArgs a) {
             dl[i] = (float)dr[i] + bias;
             z[i] = gated ? (float)zr[i] : 0.0f;
         }
-        if (t + TT < p.t1) fetch(t + TT);
+        if (t + TT < p.t1) fetch();
 #pragma unroll
         for (int i = 0; i < TT; ++i) {
             if (t + i >= p.t1) break;
-            const uniform_f32 row = bc + (t + i) * 2 * NS;
             if (a.softplus) dl[i] = softplus(dl[i]);
             if (starts & 1) {
                 cut = true;
@@ -182,11 +192,10 @@ __global__ __launch_bounds__(64) void scan_forward(ScanArgs a) {
                 for (int n = 0; n < NS; ++n) h[n] = 0.0f;
             }
             starts >>= 1;
-            if (!ENDS && a.marks && (t + i) % kTile<NS> == 0 && p.live) {
-                float* m = a.marks + (((int64_t)p.b * ((a.length + kTile<NS> - 1) / kTile<NS>) + (t + i) / kTile<NS>) * NS) *
-                                         a.channels + p.d;
+            if (!ENDS && marks && (kTile<NS> <= TT ? i % kTile<NS> == 0 : i == 0 && (t - p.t0) % kTile<NS> == 0)) {
 #pragma unroll
-                for (int n = 0; n < NS; ++n) m[(int64_t)n * a.channels] = h[n];
+                for (int n = 0; n < NS; ++n, marks += a.channels)
+                    if (p.live) marks[p.lane] = h[n];
             }
             const float in = dl[i] * x[i];
             if (ENDS) sum += dl[i];
@@ -201,10 +210,12 @@ __global__ __launch_bounds__(64) void scan_forward(ScanArgs a) {
                         y0 = __builtin_fmaf(h[n], row[NS + n], y0);
                 }
             }
+            row += 2 * NS;
             if (!ENDS) {
                 float y = y0 + y1;
                 if (gated) y *= z[i] * sigmoid(z[i]);
-                if (p.live) yp[(t + i) * a.y_t] = (T)y;
+                if (p.live) yp[p.lane] = (T)y;
+                yp += a.y_t;
             }
         }
     }
@@ -236,11 +247,22 @@ __global__ __launch_bounds__(256) void scan_join(float* ends, const float* prods
     float carry = seed && n < N ? seed[(b * channels + d) * N + n] : 0.0f;
     float* e = ends + b * chunks * row + r;
     const float* q = prods + b * chunks * row + r;
-    for (int k = 0; k < chunks; ++k) {
-        const int64_t s = (REV ? chunks - 1 - k : k) * row;
-        const float end = e[s], prod = q[s];
-        e[s] = carry;
-        carry = prod == 0.0f ? end : __builtin_fmaf(prod, carry, end);   // a cut keeps nothing, not even a NaN
+    constexpr int AHEAD = 16;   // chunks whose loads are in flight together
+    for (int k = 0; k < chunks; k += AHEAD) {
+        float end[AHEAD], prod[AHEAD];
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) {
+            const int c = k + j < chunks ? k + j : chunks - 1;
+            const int64_t s = (REV ? chunks - 1 - c : c) * row;
+            end[j] = e[s];
+            prod[j] = q[s];
+        }
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) {
+            if (k + j >= chunks) break;
+            e[(REV ? chunks - 1 - (k + j) : k + j) * row] = carry;
+            carry = prod[j] == 0.0f ? end[j] : __builtin_fmaf(prod[j], carry, end[j]);   // a cut keeps nothing, not even a NaN
+        }
     }
 }
 
@@ -263,20 +285,35 @@ __device__ inline float fold(float a, float b) {
         constexpr int ctrl = LEVEL == 2 ? 0x128 : LEVEL == 3 ? 0x141 : LEVEL == 4 ? 0x4E : 0xB1;
         const bool hi = threadIdx.x & (32 >> LEVEL);
         const float keep = hi ? b : a, give = hi ? a : b;
-        const int got = __builtin_amdgcn_update_dpp(0, __float_as_int(give), ctrl, 0xf, 0xf, true);
+        const int got = __builtin_amdgcn_mov_dpp(__float_as_int(give), ctrl, 0xf, 0xf, true);
         return keep + __int_as_float(got);
     }
 }
 
+// The sums of f(base) .. f(base + 2^HEIGHT - 1), each in the lane whose bits 5,
+// 4, .. are its index's bits 0, 1, ..; f is called in order, and what is folded
+// away is gone from the registers.
+template <int HEIGHT, class F>
+__device__ __forceinline__ float folded(F& f, int base) {
+    if constexpr (HEIGHT == 0) {
+        return f(base);
+    } else {
+        const float lo = folded<HEIGHT - 1>(f, base);
+        const float hi = folded<HEIGHT - 1>(f, base + (1 << (HEIGHT - 1)));
+        return fold<HEIGHT - 1>(lo, hi);
+    }
+}
+
+// The same of values already folded up to LEVEL.
 template <int LEVEL, int COUNT>
-__device__ inline float fold_all(float (&v)[COUNT]) {
+__device__ __forceinline__ float fold_rest(float (&v)[COUNT]) {
     if constexpr (COUNT == 1) {
         return v[0];
     } else {
         float r[COUNT / 2];
 #pragma unroll
         for (int i = 0; i < COUNT / 2; ++i) r[i] = fold<LEVEL>(v[2 * i], v[2 * i + 1]);
-        return fold_all<LEVEL + 1>(r);
+        return fold_rest<LEVEL + 1>(r);
     }
 }
 
@@ -330,10 +367,15 @@ __global__ __launch_bounds__(64) void scan_backward_ends(ScanArgs a, GradArgs ga
     }
 }
 
+// The walk back goes by tiles of half the marks' distance, whose kept states
+// (64 registers) it works out forwards first: the lower tile of a pair from the
+// mark, the upper one by going over the lower one too (an eighth more work; with
+// whole tiles' 128 registers the kernel spills and takes six times as long).
 template <typename T, int NS>
 __global__ __launch_bounds__(64, 2) void scan_backward(ScanArgs a, GradArgs ga) {
-    constexpr int TT = kTile<NS>;
+    constexpr int TT = kTile<NS> / 2;
     constexpr int G = 64 / (2 * NS);   // steps whose 2 NS sums fill the lanes
+    static_assert(G <= TT, "a tile's sums fill the lanes");
     const Place p = place_of(a);
     float A2[NS], g[NS], dA[NS];
     load_rates<NS>(a, p.d, A2);
@@ -341,97 +383,154 @@ __global__ __launch_bounds__(64, 2) void scan_backward(ScanArgs a, GradArgs ga) 
 #pragma unroll
     for (int n = 0; n < NS; ++n) {
         dA[n] = 0.0f;
-        if (a.chunks > 1)
-            g[n] = ga.ends[slot + (int64_t)n * a.channels];
-        else
-            g[n] = ga.dstate_out && n < a.N ? ga.dstate_out[((int64_t)p.b * a.channels + p.d) * a.N + n] : 0.0f;
+        g[n] = 0.0f;
+        if (p.live) {
+            if (a.chunks > 1)
+                g[n] = ga.ends[slot + (int64_t)n * a.channels];
+            else if (ga.dstate_out && n < a.N)
+                g[n] = ga.dstate_out[((int64_t)p.b * a.channels + p.d) * a.N + n];
+        }
     }
     const float skip = a.skip ? a.skip[p.d] : 0.0f, bias = a.bias ? a.bias[p.d] : 0.0f;
     float dskip = 0.0f, dbias = 0.0f;
-    const T* xp = (const T*)a.x.p + p.b * a.x.b + p.d;
-    const T* dp = (const T*)a.dt.p + p.b * a.dt.b + p.d;
-    const T* op = (const T*)ga.dout.p + p.b * ga.dout.b + p.d;
     const bool gated = a.z.p != nullptr;
-    const T* zp = gated ? (const T*)a.z.p + p.b * a.z.b + p.d : xp;
-    const int64_t dense = (int64_t)p.b * a.length * a.channels + p.d;
+    // rows of the wave's channels: a uniform address and the lane
+    const T* xp = (const T*)a.x.p + p.b * a.x.b + p.base;
+    const T* dp = (const T*)a.dt.p + p.b * a.dt.b + p.base;
+    const T* op = (const T*)ga.dout.p + p.b * ga.dout.b + p.base;
+    const T* zp = gated ? (const T*)a.z.p + p.b * a.z.b + p.base : xp;
+    const int64_t zt = gated ? a.z.t : 0;
+    const int64_t dense = (int64_t)p.b * a.length * a.channels + p.base;
     T* dxp = (T*)ga.dx + dense;
     T* ddp = (T*)ga.ddt + dense;
     T* dzp = gated ? (T*)ga.dz + dense : nullptr;
     const uniform_f32 bc = (uniform_f32)(uintptr_t)(a.bc + (int64_t)p.b * a.length * 2 * NS);
-    const int64_t tiles = (a.length + TT - 1) / TT;
+    const int64_t tiles = (a.length + kTile<NS> - 1) / kTile<NS>;
     // the sums' place: lane l ends up with the value whose index is l's bits turned round
     const int k = (int)(__builtin_bitreverse32(threadIdx.x) >> 26);
-    float* part = ga.bc_part + (((int64_t)p.blk * a.batch + p.b) * a.length + k / (2 * NS)) * 2 * NS + k % (2 * NS);
+    float* part = ga.bc_part + ((int64_t)p.blk * a.batch + p.b) * a.length * 2 * NS;
     uint64_t starts = 0;
     int64_t from = p.t1;
 
+#pragma unroll 1
     for (int64_t t = p.t0 + (p.t1 - 1 - p.t0) / TT * TT; t >= p.t0; t -= TT) {
+        const bool upper = (t - p.t0) & TT;
+        const int steps = p.t1 - t < TT ? (int)(p.t1 - t) : TT;
         if (a.resets && t < from) {
             from = p.t0 + (t - p.t0) / 64 * 64;
             starts = resets_at(a, p.b, from, p.t1);
         }
         const unsigned cuts = (unsigned)(starts >> (t - from));
-        float w[TT][NS], dl[TT], x[TT], dy[TT], sg[TT];
-        float h[NS];
-        const float* m = a.marks + (((int64_t)p.b * tiles + t / TT) * NS) * a.channels + p.d;
+        T xr[TT], dr[TT], orr[TT], zr[TT];
+        {
+            const T *x0 = xp + t * a.x.t, *d0 = dp + t * a.dt.t, *o0 = op + t * ga.dout.t, *z0 = zp + t * zt;
 #pragma unroll
-        for (int n = 0; n < NS; ++n) h[n] = m[(int64_t)n * a.channels];
+            for (int i = 0; i < TT; ++i) {
+                dr[i] = d0[p.lane];
+                xr[i] = x0[p.lane];
+                orr[i] = o0[p.lane];
+                zr[i] = z0[p.lane];
+                if (i + 1 < steps) x0 += a.x.t, d0 += a.dt.t, o0 += ga.dout.t, z0 += zt;   // steps past the end read the last one
+            }
+        }
+        float h[NS];
+        const float* m = a.marks + (((int64_t)p.b * tiles + t / kTile<NS>) * NS) * a.channels + p.base;
+#pragma unroll
+        for (int n = 0; n < NS; ++n, m += a.channels) h[n] = m[p.lane];
+        if (upper) {
+            const unsigned before = (unsigned)(starts >> (t - TT - from));
+            const T *x0 = xp + (t - TT) * a.x.t, *d0 = dp + (t - TT) * a.dt.t;
+            T xb[TT], db[TT];
+#pragma unroll
+            for (int i = 0; i < TT; ++i, x0 += a.x.t, d0 += a.dt.t) {
+                db[i] = d0[p.lane];
+                xb[i] = x0[p.lane];
+            }
+            uniform_f32 row = bc + (t - TT) * 2 * NS;
+#pragma unroll
+            for (int i = 0; i < TT; ++i, row += 2 * NS) {
+                float v = (float)db[i] + bias;
+                if (a.softplus) v = softplus(v);
+                const float u = v * (float)xb[i];
+                if (before >> i & 1) {
+#pragma unroll
+                    for (int n = 0; n < NS; ++n) h[n] = 0.0f;
+                }
+#pragma unroll
+                for (int n = 0; n < NS; ++n) h[n] = __builtin_fmaf(exp2_fast(v * A2[n]), h[n], u * row[n]);
+            }
+        }
+        float w[TT][NS], dl[TT], x[TT], dy[TT], sg[TT];
         // forwards through the tile: w = what each step keeps of its past.
-        // Steps past the end are steps of nothing: D = 0, x = 0, dy = 0.
+        // Steps past the end, and lanes past the last channel, are of nothing:
+        // D = 0, x = 0, dy = 0.
+        const uniform_f32 rows = bc + t * 2 * NS;
 #pragma unroll
         for (int i = 0; i < TT; ++i) {
-            const bool in = t + i < p.t1;
-            const int64_t q = in ? t + i : p.t1 - 1;
-            const uniform_f32 row = bc + q * 2 * NS;
-            float v = (float)dp[q * a.dt.t] + bias;
+            const bool in = i < steps && p.live;
+            const uniform_f32 row = rows + (i < steps ? i : 0) * 2 * NS;
+            float v = (float)dr[i] + bias;
             sg[i] = a.softplus ? sigmoid(v) : 1.0f;
             if (a.softplus) v = softplus(v);
             dl[i] = in ? v : 0.0f;
-            x[i] = in ? (float)xp[q * a.x.t] : 0.0f;
-            const float dout = in ? (float)op[q * ga.dout.t] : 0.0f;
+            x[i] = in ? (float)xr[i] : 0.0f;
+            const float dout = in ? (float)orr[i] : 0.0f;
             const float u = dl[i] * x[i];
             if (cuts >> i & 1) {
 #pragma unroll
                 for (int n = 0; n < NS; ++n) h[n] = 0.0f;
             }
-            float y0 = skip * x[i], y1 = 0.0f;
+            dy[i] = dout;
+            if (gated) {
+                float y0 = skip * x[i], y1 = 0.0f;
 #pragma unroll
-            for (int n = 0; n < NS; ++n) {
-                w[i][n] = exp2_fast(dl[i] * A2[n]) * h[n];
-                h[n] = __builtin_fmaf(u, row[n], w[i][n]);
-                if (gated) {
+                for (int n = 0; n < NS; ++n) {
+                    w[i][n] = exp2_fast(dl[i] * A2[n]) * h[n];
+                    h[n] = __builtin_fmaf(u, row[n], w[i][n]);
                     if (n & 1)
                         y1 = __builtin_fmaf(h[n], row[NS + n], y1);
                     else
                         y0 = __builtin_fmaf(h[n], row[NS + n], y0);
                 }
-            }
-            dy[i] = dout;
-            if (gated) {
-                const float z = (float)zp[q * a.z.t], s = sigmoid(z);
-                dy[i] = dout * z * s;
-                if (in && p.live) dzp[q * a.channels] = (T)(dout * (y0 + y1) * s * __builtin_fmaf(z, 1.0f - s, 1.0f));
+                const float z = (float)zr[i], s = sigmoid(z);
+                dy[i] = in ? dout * z * s : 0.0f;
+                if (in) {
+                    T* row_dz = dzp + (t + i) * a.channels;
+                    row_dz[p.lane] = (T)(dout * (y0 + y1) * s * __builtin_fmaf(z, 1.0f - s, 1.0f));
+                }
+            } else {
+#pragma unroll
+                for (int n = 0; n < NS; ++n) {
+                    w[i][n] = exp2_fast(dl[i] * A2[n]) * h[n];
+                    h[n] = __builtin_fmaf(u, row[n], w[i][n]);
+                }
             }
         }
         float r[G];
+        // B and C are loaded anew: held since the walk forwards, a tile's rows
+        // would not fit the SGPRs
+        uint64_t again = (uint64_t)(uintptr_t)rows;
+        asm volatile("" : "+s"(again));
+        const uniform_f32 rows2 = (uniform_f32)(uintptr_t)again;
 #pragma unroll
         for (int i = TT - 1; i >= 0; --i) {
-            const bool in = t + i < p.t1;
-            const int64_t q = in ? t + i : p.t1 - 1;
-            const uniform_f32 row = bc + q * 2 * NS;
+            const bool in = i < steps && p.live;
+            const uniform_f32 row = rows2 + (i < steps ? i : 0) * 2 * NS;
             const float u = dl[i] * x[i];
-            float v[2 * NS], gb = 0.0f, ga_ = 0.0f;
-#pragma unroll
-            for (int n = 0; n < NS; ++n) {
+            float gb = 0.0f, ga_ = 0.0f;
+            auto value = [&](int q) {
+                const int n = q & (NS - 1);
+                if (q >= NS) return dy[i] * __builtin_fmaf(u, row[n], w[i][n]);   // dy h: of dC
                 g[n] = __builtin_fmaf(dy[i], row[NS + n], g[n]);
-                v[n] = p.live ? g[n] * u : 0.0f;
-                v[NS + n] = p.live ? dy[i] * __builtin_fmaf(u, row[n], w[i][n]) : 0.0f;
+                const float of_b = g[n] * u;
                 gb = __builtin_fmaf(g[n], row[n], gb);
                 const float kept = g[n] * w[i][n];
                 ga_ = __builtin_fmaf(kept, A2[n], ga_);
                 dA[n] = __builtin_fmaf(kept, dl[i], dA[n]);
                 g[n] *= exp2_fast(dl[i] * A2[n]);
-            }
+                return of_b;
+            };
+            r[i % G] = folded<log2_of(2 * NS)>(value, 0);
             if (cuts >> i & 1) {
 #pragma unroll
                 for (int n = 0; n < NS; ++n) g[n] = 0.0f;
@@ -440,15 +539,13 @@ __global__ __launch_bounds__(64, 2) void scan_backward(ScanArgs a, GradArgs ga) 
             if (in) {
                 dskip = __builtin_fmaf(dy[i], x[i], dskip);
                 dbias += ddl;
-                if (p.live) {
-                    dxp[q * a.channels] = (T)__builtin_fmaf(dl[i], gb, skip * dy[i]);
-                    ddp[q * a.channels] = (T)ddl;
-                }
+                T *row_dx = dxp + (t + i) * a.channels, *row_dd = ddp + (t + i) * a.channels;
+                row_dx[p.lane] = (T)__builtin_fmaf(dl[i], gb, skip * dy[i]);
+                row_dd[p.lane] = (T)ddl;
             }
-            r[i % G] = fold_all<0>(v);
             if (i % G == 0) {
-                const float s = fold_all<log2_of(2 * NS)>(r);
-                if (t + i + k / (2 * NS) < p.t1) part[(t + i) * 2 * NS] = s;
+                const float s = fold_rest<log2_of(2 * NS)>(r);
+                if (i + k / (2 * NS) < steps) (part + (t + i) * 2 * NS)[k] = s;
             }
         }
     }
@@ -612,7 +709,7 @@ int32_t check_scan(const char* fn, const SdfrScan* s) {
     if (s->states < 1 || s->states > kMaxStates)
         return rec_fail(-2, "%s: states must be 1 to %d (got %d)", fn, kMaxStates, s->states);
     if (!rec_float(s->dtype)) return rec_fail(-3, "%s: dtype must be f32, f16 or bf16 (got %d)", fn, s->dtype);
-    if (s->channels > (1 << 24) || s->length > ((int64_t)1 << 40) ||
+    if (s->channels > (1 << 24) || s->length > 0x7fffff00 ||
         (int64_t)s->batch * ((s->channels + 63) / 64) > 0x3fffffff)
         return rec_fail(-2, "%s: sizes too large", fn);
     if (!s->A) return rec_fail(-1, "%s: null rates", fn);
