@@ -108,11 +108,50 @@ __device__ inline Place place_of(const ScanArgs& a) {
     return p;
 }
 
+// A lane's N numbers from a row of N, padded with zeros. No branch a number:
+// all the loads go out together.
 template <int NS>
-__device__ inline void load_rates(const ScanArgs& a, int d, float (&A2)[NS]) {
+__device__ __forceinline__ void load_states(const float* row, int N, float (&v)[NS]) {
 #pragma unroll
-    for (int n = 0; n < NS; ++n) A2[n] = n < a.N ? a.A[(int64_t)d * a.N + n] * kLog2e : 0.0f;
+    for (int n = 0; n < NS; ++n) {
+        const float r = row[n < N ? n : N - 1];
+        v[n] = n < N ? r : 0.0f;
+    }
 }
+
+template <int NS>
+__device__ __forceinline__ void load_rates(const ScanArgs& a, int d, float (&A2)[NS]) {
+    load_states<NS>(a.A + (int64_t)d * a.N, a.N, A2);
+#pragma unroll
+    for (int n = 0; n < NS; ++n) A2[n] *= kLog2e;
+}
+
+// Where a chunk's walk begins: at what scan_join left for it, or at the given
+// state, or at zero.
+template <int NS>
+__device__ __forceinline__ void load_start(const ScanArgs& a, const Place& p, const float* ends, const float* given,
+                                           float (&v)[NS]) {
+    if (a.chunks > 1) {
+        const float* e = ends + (((int64_t)p.b * a.chunks + p.s) * NS) * a.channels + p.d;
+#pragma unroll
+        for (int n = 0; n < NS; ++n) v[n] = e[(int64_t)n * a.channels];
+    } else if (given) {
+        load_states<NS>(given + ((int64_t)p.b * a.channels + p.d) * a.N, a.N, v);
+    } else {
+#pragma unroll
+        for (int n = 0; n < NS; ++n) v[n] = 0.0f;
+    }
+}
+
+// One step's packed B and C, uniform over the wave.
+template <int NS>
+struct BC {
+    float v[2 * NS];
+    __device__ __forceinline__ explicit BC(uniform_f32 row) {
+#pragma unroll
+        for (int n = 0; n < 2 * NS; ++n) v[n] = row[n];
+    }
+};
 
 // ---- packing B and C -------------------------------------------------------
 template <typename T, int NS>
@@ -128,32 +167,34 @@ __global__ __launch_bounds__(256) void bc_pack(Rows B, Rows C, float* __restrict
 }
 
 // ---- forward ---------------------------------------------------------------
-// ENDS: only the chunk's end state from zero and the product of its decays.
-template <typename T, int NS, bool ENDS>
+enum { kEnds, kPlain, kGated };
+
+// kEnds: only the chunk's end state from zero and the product of its decays.
+//
+// Two copies of the eight steps: one without a branch, in which the next step's
+// B and C are on their way while this one computes, and one for tiles that a
+// sequence begins in or that are not whole. With a branch a step the waits for
+// the scalar loads took half the kernel's time.
+template <typename T, int NS, int MODE>
 __global__ __launch_bounds__(64) void scan_forward(ScanArgs a) {
     constexpr int TT = 8;
+    constexpr bool GATED = MODE == kGated, ENDS = MODE == kEnds;
     const Place p = place_of(a);
     float A2[NS], h[NS];
     load_rates<NS>(a, p.d, A2);
-    const int64_t slot = (((int64_t)p.b * a.chunks + p.s) * NS) * a.channels + p.d;
+    if constexpr (ENDS) {
 #pragma unroll
-    for (int n = 0; n < NS; ++n) {
-        if (ENDS)
-            h[n] = 0.0f;
-        else if (a.chunks > 1)
-            h[n] = a.ends[slot + (int64_t)n * a.channels];
-        else
-            h[n] = a.state && n < a.N ? a.state[((int64_t)p.b * a.channels + p.d) * a.N + n] : 0.0f;
+        for (int n = 0; n < NS; ++n) h[n] = 0.0f;
+    } else {
+        load_start<NS>(a, p, a.ends, a.state, h);
     }
     const float skip = a.skip ? a.skip[p.d] : 0.0f, bias = a.bias ? a.bias[p.d] : 0.0f;
-    const bool gated = !ENDS && a.z.p;
     // rows of the wave's channels: a uniform address and the lane
     const T* xp = (const T*)a.x.p + p.b * a.x.b + p.t0 * a.x.t + p.base;
     const T* dp = (const T*)a.dt.p + p.b * a.dt.b + p.t0 * a.dt.t + p.base;
-    const T* zp = gated ? (const T*)a.z.p + p.b * a.z.b + p.t0 * a.z.t + p.base : xp;
-    const int64_t zt = gated ? a.z.t : 0;
+    const T* zp = GATED ? (const T*)a.z.p + p.b * a.z.b + p.t0 * a.z.t + p.base : nullptr;
     T* yp = ENDS ? nullptr : (T*)a.y + p.b * a.y_b + p.t0 * a.y_t + p.base;
-    uniform_f32 row = (uniform_f32)(uintptr_t)(a.bc + ((int64_t)p.b * a.length + p.t0) * 2 * NS);
+    uniform_f32 rows = (uniform_f32)(uintptr_t)(a.bc + ((int64_t)p.b * a.length + p.t0) * 2 * NS);
     float* marks = !ENDS && a.marks ? a.marks + (((int64_t)p.b * ((a.length + kTile<NS> - 1) / kTile<NS>) + p.t0 / kTile<NS>) * NS) *
                                                     a.channels + p.base
                                     : nullptr;
@@ -161,66 +202,91 @@ __global__ __launch_bounds__(64) void scan_forward(ScanArgs a) {
     bool cut = false;
     float sum = 0.0f;
     T xr[TT], dr[TT], zr[TT];
-    int left = (int)(p.t1 - p.t0);   // steps not yet fetched (a chunk is short, a whole sequence of 2^31 steps too long)
+    const int total = (int)(p.t1 - p.t0);
+    int left = total;   // steps not yet fetched
     auto fetch = [&]() {
 #pragma unroll
         for (int i = 0; i < TT; ++i) {
             xr[i] = xp[p.lane];
             dr[i] = dp[p.lane];
-            if (!ENDS) zr[i] = zp[p.lane];
-            if (--left > 0) xp += a.x.t, dp += a.dt.t, zp += zt;   // past the end the last one again
+            if (GATED) zr[i] = zp[p.lane];
+            --left;
+            xp += left > 0 ? a.x.t : 0;   // past the end the last one again
+            dp += left > 0 ? a.dt.t : 0;
+            if (GATED) zp += left > 0 ? a.z.t : 0;
+        }
+    };
+    auto mark = [&]() {
+#pragma unroll
+        for (int n = 0; n < NS; ++n, marks += a.channels) marks[p.lane] = h[n];   // lanes past the end write what the last one does
+    };
+    auto step = [&](float dl, float x, float z, const BC<NS>& row) {
+        const float in = dl * x;
+        if (ENDS) sum += dl;
+        float y0 = skip * x, y1 = 0.0f;
+#pragma unroll
+        for (int n = 0; n < NS; ++n) {
+            h[n] = __builtin_fmaf(exp2_fast(dl * A2[n]), h[n], in * row.v[n]);
+            if (!ENDS) {
+                if (n & 1)
+                    y1 = __builtin_fmaf(h[n], row.v[NS + n], y1);
+                else
+                    y0 = __builtin_fmaf(h[n], row.v[NS + n], y0);
+            }
+        }
+        if (!ENDS) {
+            float y = y0 + y1;
+            if (GATED) y *= z * sigmoid(z);
+            yp[p.lane] = (T)y;
+            yp += a.y_t;
         }
     };
     fetch();
-    for (int64_t t = p.t0; t < p.t1; t += TT) {
-        if (a.resets && ((t - p.t0) & 63) == 0) starts = resets_at(a, p.b, t, p.t1);
+#pragma unroll 1
+    for (int t = 0; t < total; t += TT) {
+        if (a.resets && (t & 63) == 0) starts = resets_at(a, p.b, p.t0 + t, p.t1);
         float x[TT], dl[TT], z[TT];
 #pragma unroll
         for (int i = 0; i < TT; ++i) {
             x[i] = (float)xr[i];
             dl[i] = (float)dr[i] + bias;
-            z[i] = gated ? (float)zr[i] : 0.0f;
+            z[i] = GATED ? (float)zr[i] : 0.0f;
         }
-        if (t + TT < p.t1) fetch();
+        if (a.softplus) {
 #pragma unroll
-        for (int i = 0; i < TT; ++i) {
-            if (t + i >= p.t1) break;
-            if (a.softplus) dl[i] = softplus(dl[i]);
-            if (starts & 1) {
-                cut = true;
+            for (int i = 0; i < TT; ++i) dl[i] = softplus(dl[i]);
+        }
+        if (t + TT < total) fetch();
+        const bool marking = !ENDS && marks;
+        if (t + TT <= total && !(starts & ((1 << TT) - 1))) {
+            BC<NS> row(rows);
+            if (marking && t % kTile<NS> == 0) mark();
 #pragma unroll
-                for (int n = 0; n < NS; ++n) h[n] = 0.0f;
+            for (int i = 0; i < TT; ++i) {
+                if (kTile<NS> < TT && i > 0 && i % kTile<NS> == 0 && marking) mark();
+                const BC<NS> next(rows + (i + 1) * 2 * NS);   // one row past the last is in the workspace too
+                step(dl[i], x[i], z[i], row);
+                row = next;
             }
-            starts >>= 1;
-            if (!ENDS && marks && (kTile<NS> <= TT ? i % kTile<NS> == 0 : i == 0 && (t - p.t0) % kTile<NS> == 0)) {
+        } else {
 #pragma unroll
-                for (int n = 0; n < NS; ++n, marks += a.channels)
-                    if (p.live) marks[p.lane] = h[n];
-            }
-            const float in = dl[i] * x[i];
-            if (ENDS) sum += dl[i];
-            float y0 = skip * x[i], y1 = 0.0f;
+            for (int i = 0; i < TT; ++i) {
+                if (t + i >= total) break;
+                if (starts >> i & 1) {
+                    cut = true;
 #pragma unroll
-            for (int n = 0; n < NS; ++n) {
-                h[n] = __builtin_fmaf(exp2_fast(dl[i] * A2[n]), h[n], in * row[n]);
-                if (!ENDS) {
-                    if (n & 1)
-                        y1 = __builtin_fmaf(h[n], row[NS + n], y1);
-                    else
-                        y0 = __builtin_fmaf(h[n], row[NS + n], y0);
+                    for (int n = 0; n < NS; ++n) h[n] = 0.0f;
                 }
-            }
-            row += 2 * NS;
-            if (!ENDS) {
-                float y = y0 + y1;
-                if (gated) y *= z[i] * sigmoid(z[i]);
-                if (p.live) yp[p.lane] = (T)y;
-                yp += a.y_t;
+                if (marking && (t + i) % kTile<NS> == 0) mark();
+                step(dl[i], x[i], z[i], BC<NS>(rows + i * 2 * NS));
             }
         }
+        rows += TT * 2 * NS;
+        starts >>= TT;
     }
     if (!p.live) return;
     if (ENDS) {
+        const int64_t slot = (((int64_t)p.b * a.chunks + p.s) * NS) * a.channels + p.d;
 #pragma unroll
         for (int n = 0; n < NS; ++n) {
             a.ends[slot + (int64_t)n * a.channels] = h[n];
@@ -371,7 +437,11 @@ __global__ __launch_bounds__(64) void scan_backward_ends(ScanArgs a, GradArgs ga
 // (64 registers) it works out forwards first: the lower tile of a pair from the
 // mark, the upper one by going over the lower one too (an eighth more work; with
 // whole tiles' 128 registers the kernel spills and takes six times as long).
-template <typename T, int NS>
+//
+// As in scan_forward there are two copies of a tile, without branches and with.
+// Lanes past the last channel repeat it, and write what it writes, but add
+// nothing to the sums over channels.
+template <typename T, int NS, bool GATED>
 __global__ __launch_bounds__(64, 2) void scan_backward(ScanArgs a, GradArgs ga) {
     constexpr int TT = kTile<NS> / 2;
     constexpr int G = 64 / (2 * NS);   // steps whose 2 NS sums fill the lanes
@@ -379,31 +449,20 @@ __global__ __launch_bounds__(64, 2) void scan_backward(ScanArgs a, GradArgs ga) 
     const Place p = place_of(a);
     float A2[NS], g[NS], dA[NS];
     load_rates<NS>(a, p.d, A2);
-    const int64_t slot = (((int64_t)p.b * a.chunks + p.s) * NS) * a.channels + p.d;
+    load_start<NS>(a, p, ga.ends, ga.dstate_out, g);
 #pragma unroll
-    for (int n = 0; n < NS; ++n) {
-        dA[n] = 0.0f;
-        g[n] = 0.0f;
-        if (p.live) {
-            if (a.chunks > 1)
-                g[n] = ga.ends[slot + (int64_t)n * a.channels];
-            else if (ga.dstate_out && n < a.N)
-                g[n] = ga.dstate_out[((int64_t)p.b * a.channels + p.d) * a.N + n];
-        }
-    }
+    for (int n = 0; n < NS; ++n) dA[n] = 0.0f;
     const float skip = a.skip ? a.skip[p.d] : 0.0f, bias = a.bias ? a.bias[p.d] : 0.0f;
     float dskip = 0.0f, dbias = 0.0f;
-    const bool gated = a.z.p != nullptr;
     // rows of the wave's channels: a uniform address and the lane
     const T* xp = (const T*)a.x.p + p.b * a.x.b + p.base;
     const T* dp = (const T*)a.dt.p + p.b * a.dt.b + p.base;
     const T* op = (const T*)ga.dout.p + p.b * ga.dout.b + p.base;
-    const T* zp = gated ? (const T*)a.z.p + p.b * a.z.b + p.base : xp;
-    const int64_t zt = gated ? a.z.t : 0;
+    const T* zp = GATED ? (const T*)a.z.p + p.b * a.z.b + p.base : nullptr;
     const int64_t dense = (int64_t)p.b * a.length * a.channels + p.base;
     T* dxp = (T*)ga.dx + dense;
     T* ddp = (T*)ga.ddt + dense;
-    T* dzp = gated ? (T*)ga.dz + dense : nullptr;
+    T* dzp = GATED ? (T*)ga.dz + dense : nullptr;
     const uniform_f32 bc = (uniform_f32)(uintptr_t)(a.bc + (int64_t)p.b * a.length * 2 * NS);
     const int64_t tiles = (a.length + kTile<NS> - 1) / kTile<NS>;
     // the sums' place: lane l ends up with the value whose index is l's bits turned round
@@ -412,25 +471,22 @@ __global__ __launch_bounds__(64, 2) void scan_backward(ScanArgs a, GradArgs ga) 
     uint64_t starts = 0;
     int64_t from = p.t1;
 
-#pragma unroll 1
-    for (int64_t t = p.t0 + (p.t1 - 1 - p.t0) / TT * TT; t >= p.t0; t -= TT) {
-        const bool upper = (t - p.t0) & TT;
-        const int steps = p.t1 - t < TT ? (int)(p.t1 - t) : TT;
-        if (a.resets && t < from) {
-            from = p.t0 + (t - p.t0) / 64 * 64;
-            starts = resets_at(a, p.b, from, p.t1);
-        }
-        const unsigned cuts = (unsigned)(starts >> (t - from));
+    auto tile = [&](auto slow, int64_t t, bool upper, int steps, unsigned cuts, unsigned before) {
+        constexpr bool SLOW = decltype(slow)::value;
         T xr[TT], dr[TT], orr[TT], zr[TT];
         {
-            const T *x0 = xp + t * a.x.t, *d0 = dp + t * a.dt.t, *o0 = op + t * ga.dout.t, *z0 = zp + t * zt;
+            const T *x0 = xp + t * a.x.t, *d0 = dp + t * a.dt.t, *o0 = op + t * ga.dout.t, *z0 = GATED ? zp + t * a.z.t : nullptr;
 #pragma unroll
             for (int i = 0; i < TT; ++i) {
                 dr[i] = d0[p.lane];
                 xr[i] = x0[p.lane];
                 orr[i] = o0[p.lane];
-                zr[i] = z0[p.lane];
-                if (i + 1 < steps) x0 += a.x.t, d0 += a.dt.t, o0 += ga.dout.t, z0 += zt;   // steps past the end read the last one
+                if (GATED) zr[i] = z0[p.lane];
+                const bool more = !SLOW || i + 1 < steps;   // steps past the end read the last one
+                x0 += more ? a.x.t : 0;
+                d0 += more ? a.dt.t : 0;
+                o0 += more ? ga.dout.t : 0;
+                if (GATED) z0 += more ? a.z.t : 0;
             }
         }
         float h[NS];
@@ -438,7 +494,6 @@ __global__ __launch_bounds__(64, 2) void scan_backward(ScanArgs a, GradArgs ga) 
 #pragma unroll
         for (int n = 0; n < NS; ++n, m += a.channels) h[n] = m[p.lane];
         if (upper) {
-            const unsigned before = (unsigned)(starts >> (t - TT - from));
             const T *x0 = xp + (t - TT) * a.x.t, *d0 = dp + (t - TT) * a.dt.t;
             T xb[TT], db[TT];
 #pragma unroll
@@ -446,64 +501,72 @@ __global__ __launch_bounds__(64, 2) void scan_backward(ScanArgs a, GradArgs ga) 
                 db[i] = d0[p.lane];
                 xb[i] = x0[p.lane];
             }
-            uniform_f32 row = bc + (t - TT) * 2 * NS;
+            float v[TT];
 #pragma unroll
-            for (int i = 0; i < TT; ++i, row += 2 * NS) {
-                float v = (float)db[i] + bias;
-                if (a.softplus) v = softplus(v);
-                const float u = v * (float)xb[i];
-                if (before >> i & 1) {
+            for (int i = 0; i < TT; ++i) v[i] = (float)db[i] + bias;
+            if (a.softplus) {
+#pragma unroll
+                for (int i = 0; i < TT; ++i) v[i] = softplus(v[i]);
+            }
+            const uniform_f32 row = bc + (t - TT) * 2 * NS;
+#pragma unroll
+            for (int i = 0; i < TT; ++i) {
+                const float u = v[i] * (float)xb[i];
+                if (SLOW && before >> i & 1) {
 #pragma unroll
                     for (int n = 0; n < NS; ++n) h[n] = 0.0f;
                 }
 #pragma unroll
-                for (int n = 0; n < NS; ++n) h[n] = __builtin_fmaf(exp2_fast(v * A2[n]), h[n], u * row[n]);
+                for (int n = 0; n < NS; ++n)
+                    h[n] = __builtin_fmaf(exp2_fast(v[i] * A2[n]), h[n], u * row[i * 2 * NS + n]);
             }
         }
         float w[TT][NS], dl[TT], x[TT], dy[TT], sg[TT];
+#pragma unroll
+        for (int i = 0; i < TT; ++i) dl[i] = (float)dr[i] + bias;
+        if (a.softplus) {
+#pragma unroll
+            for (int i = 0; i < TT; ++i) {
+                sg[i] = sigmoid(dl[i]);
+                dl[i] = softplus(dl[i]);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < TT; ++i) sg[i] = 1.0f;
+        }
         // forwards through the tile: w = what each step keeps of its past.
-        // Steps past the end, and lanes past the last channel, are of nothing:
-        // D = 0, x = 0, dy = 0.
+        // Steps past the end are of nothing: D = 0, x = 0, dy = 0.
         const uniform_f32 rows = bc + t * 2 * NS;
 #pragma unroll
         for (int i = 0; i < TT; ++i) {
-            const bool in = i < steps && p.live;
-            const uniform_f32 row = rows + (i < steps ? i : 0) * 2 * NS;
-            float v = (float)dr[i] + bias;
-            sg[i] = a.softplus ? sigmoid(v) : 1.0f;
-            if (a.softplus) v = softplus(v);
-            dl[i] = in ? v : 0.0f;
+            const bool in = !SLOW || i < steps;
+            const uniform_f32 row = rows + (in ? i : 0) * 2 * NS;
+            if (SLOW && !in) dl[i] = 0.0f;
             x[i] = in ? (float)xr[i] : 0.0f;
             const float dout = in ? (float)orr[i] : 0.0f;
             const float u = dl[i] * x[i];
-            if (cuts >> i & 1) {
+            if (SLOW && cuts >> i & 1) {
 #pragma unroll
                 for (int n = 0; n < NS; ++n) h[n] = 0.0f;
             }
-            dy[i] = dout;
-            if (gated) {
-                float y0 = skip * x[i], y1 = 0.0f;
+            float y0 = skip * x[i], y1 = 0.0f;
 #pragma unroll
-                for (int n = 0; n < NS; ++n) {
-                    w[i][n] = exp2_fast(dl[i] * A2[n]) * h[n];
-                    h[n] = __builtin_fmaf(u, row[n], w[i][n]);
+            for (int n = 0; n < NS; ++n) {
+                w[i][n] = exp2_fast(dl[i] * A2[n]) * h[n];
+                h[n] = __builtin_fmaf(u, row[n], w[i][n]);
+                if (GATED) {
                     if (n & 1)
                         y1 = __builtin_fmaf(h[n], row[NS + n], y1);
                     else
                         y0 = __builtin_fmaf(h[n], row[NS + n], y0);
                 }
+            }
+            dy[i] = dout;
+            if (GATED) {
                 const float z = (float)zr[i], s = sigmoid(z);
                 dy[i] = in ? dout * z * s : 0.0f;
-                if (in) {
-                    T* row_dz = dzp + (t + i) * a.channels;
-                    row_dz[p.lane] = (T)(dout * (y0 + y1) * s * __builtin_fmaf(z, 1.0f - s, 1.0f));
-                }
-            } else {
-#pragma unroll
-                for (int n = 0; n < NS; ++n) {
-                    w[i][n] = exp2_fast(dl[i] * A2[n]) * h[n];
-                    h[n] = __builtin_fmaf(u, row[n], w[i][n]);
-                }
+                T* row_dz = dzp + (t + i) * a.channels;
+                if (in) row_dz[p.lane] = (T)(dout * (y0 + y1) * s * __builtin_fmaf(z, 1.0f - s, 1.0f));
             }
         }
         float r[G];
@@ -514,15 +577,16 @@ __global__ __launch_bounds__(64, 2) void scan_backward(ScanArgs a, GradArgs ga) 
         const uniform_f32 rows2 = (uniform_f32)(uintptr_t)again;
 #pragma unroll
         for (int i = TT - 1; i >= 0; --i) {
-            const bool in = i < steps && p.live;
-            const uniform_f32 row = rows2 + (i < steps ? i : 0) * 2 * NS;
+            const bool in = !SLOW || i < steps;
+            const uniform_f32 row = rows2 + (in ? i : 0) * 2 * NS;
             const float u = dl[i] * x[i];
+            const float u_sum = p.live ? u : 0.0f, dy_sum = p.live ? dy[i] : 0.0f;
             float gb = 0.0f, ga_ = 0.0f;
             auto value = [&](int q) {
                 const int n = q & (NS - 1);
-                if (q >= NS) return dy[i] * __builtin_fmaf(u, row[n], w[i][n]);   // dy h: of dC
+                if (q >= NS) return dy_sum * __builtin_fmaf(u, row[n], w[i][n]);   // dy h: of dC
                 g[n] = __builtin_fmaf(dy[i], row[NS + n], g[n]);
-                const float of_b = g[n] * u;
+                const float of_b = g[n] * u_sum;
                 gb = __builtin_fmaf(g[n], row[n], gb);
                 const float kept = g[n] * w[i][n];
                 ga_ = __builtin_fmaf(kept, A2[n], ga_);
@@ -531,7 +595,7 @@ __global__ __launch_bounds__(64, 2) void scan_backward(ScanArgs a, GradArgs ga) 
                 return of_b;
             };
             r[i % G] = folded<log2_of(2 * NS)>(value, 0);
-            if (cuts >> i & 1) {
+            if (SLOW && cuts >> i & 1) {
 #pragma unroll
                 for (int n = 0; n < NS; ++n) g[n] = 0.0f;
             }
@@ -545,9 +609,26 @@ __global__ __launch_bounds__(64, 2) void scan_backward(ScanArgs a, GradArgs ga) 
             }
             if (i % G == 0) {
                 const float s = fold_rest<log2_of(2 * NS)>(r);
-                if (i + k / (2 * NS) < steps) (part + (t + i) * 2 * NS)[k] = s;
+                float* row_part = part + (t + i) * 2 * NS;
+                if (!SLOW || i + k / (2 * NS) < steps) row_part[k] = s;
             }
         }
+    };
+
+#pragma unroll 1
+    for (int64_t t = p.t0 + (p.t1 - 1 - p.t0) / TT * TT; t >= p.t0; t -= TT) {
+        const bool upper = (t - p.t0) & TT;
+        const int steps = p.t1 - t < TT ? (int)(p.t1 - t) : TT;
+        if (a.resets && t < from) {
+            from = p.t0 + (t - p.t0) / 64 * 64;
+            starts = resets_at(a, p.b, from, p.t1);
+        }
+        const unsigned cuts = (unsigned)(starts >> (t - from)) & ((1u << TT) - 1);
+        const unsigned before = upper ? (unsigned)(starts >> (t - TT - from)) & ((1u << TT) - 1) : 0;
+        if (steps == TT && !(cuts | before))
+            tile(std::false_type(), t, upper, TT, 0u, 0u);
+        else
+            tile(std::true_type(), t, upper, steps, cuts, before);
     }
     if (!p.live) return;
     float* sums = ga.sums + (((int64_t)p.b * a.chunks + p.s) * (NS + 2)) * a.channels + p.d;
@@ -693,7 +774,7 @@ Plan plan_of(const SdfrScan* s, bool grad) {
     const int64_t rows = (int64_t)s->batch * s->length;
     const int64_t ends = p.chunks > 1 ? (int64_t)s->batch * p.chunks * p.NS * s->channels * 4 : 0;
     p.bc = 0;
-    p.ends = up(rows * 2 * p.NS * 4);
+    p.ends = up((rows + 1) * 2 * p.NS * 4);   // one row past the last is loaded, not used
     p.part = p.ends + 2 * up(ends);
     p.sums = p.part + (grad ? up(rows * 2 * p.NS * 4 * p.blocks) : 0);
     p.total = p.sums + (grad ? up((int64_t)s->batch * p.chunks * (p.NS + 2) * s->channels * 4) : 0);
@@ -845,11 +926,14 @@ SDFR_API int32_t sdfr_scan(const SdfrScan* s, void* workspace, int64_t workspace
             constexpr int NS = decltype(ns)::value;
             launch_pack<T, NS>(s, a, st);
             if (p.chunks > 1) {
-                scan_forward<T, NS, true><<<(unsigned)grid, 64, 0, st>>>(a);
+                scan_forward<T, NS, kEnds><<<(unsigned)grid, 64, 0, st>>>(a);
                 scan_join<false><<<(unsigned)(((int64_t)s->batch * NS * s->channels + 255) / 256), 256, 0, st>>>(
                     a.ends, a.prods, s->state, s->batch, p.chunks, NS, s->channels, s->states);
             }
-            scan_forward<T, NS, false><<<(unsigned)grid, 64, 0, st>>>(a);
+            if (s->z)
+                scan_forward<T, NS, kGated><<<(unsigned)grid, 64, 0, st>>>(a);
+            else
+                scan_forward<T, NS, kPlain><<<(unsigned)grid, 64, 0, st>>>(a);
             return 0;
         });
     });
@@ -894,7 +978,10 @@ SDFR_API int32_t sdfr_scan_grad(const SdfrScan* s, const SdfrScanGrad* g, void* 
                 scan_join<true><<<(unsigned)(((int64_t)s->batch * NS * s->channels + 255) / 256), 256, 0, st>>>(
                     a.ends, a.prods, g->dstate_out, s->batch, p.chunks, NS, s->channels, s->states);
             }
-            scan_backward<T, NS><<<(unsigned)grid, 64, 0, st>>>(a, ga);
+            if (s->z)
+                scan_backward<T, NS, true><<<(unsigned)grid, 64, 0, st>>>(a, ga);
+            else
+                scan_backward<T, NS, false><<<(unsigned)grid, 64, 0, st>>>(a, ga);
             bc_sums<T, NS><<<(unsigned)((rows * 2 * NS + 255) / 256), 256, 0, st>>>(
                 ga.bc_part, (T*)g->dB, (T*)g->dC, rows, p.blocks, s->states);
             column_sums<<<(unsigned)(((int64_t)(NS + 2) * s->channels + 63) / 64), dim3(64, 16), 0, st>>>(
