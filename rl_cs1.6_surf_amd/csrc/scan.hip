@@ -143,7 +143,9 @@ __device__ __forceinline__ void load_start(const ScanArgs& a, const Place& p, co
     }
 }
 
-// One step's packed B and C, uniform over the wave.
+// One step's packed B and C, uniform over the wave. Two steps' fit the SGPRs up
+// to 16 states; beyond that a step loads its own.
+template <int NS> constexpr bool kAhead = NS <= 16;
 template <int NS>
 struct BC {
     float v[2 * NS];
@@ -264,7 +266,8 @@ __global__ __launch_bounds__(64) void scan_forward(ScanArgs a) {
 #pragma unroll
             for (int i = 0; i < TT; ++i) {
                 if (kTile<NS> < TT && i > 0 && i % kTile<NS> == 0 && marking) mark();
-                const BC<NS> next(rows + (i + 1) * 2 * NS);   // one row past the last is in the workspace too
+                const BC<NS> next(rows + (i + 1) * 2 * NS);            // one row past the last is in the workspace too
+                if (kAhead<NS>) __builtin_amdgcn_sched_barrier(0);   // sent off here, waited for a step later
                 step(dl[i], x[i], z[i], row);
                 row = next;
             }
@@ -385,43 +388,94 @@ __device__ __forceinline__ float fold_rest(float (&v)[COUNT]) {
 
 constexpr int log2_of(int v) { return v <= 1 ? 0 : 1 + log2_of(v / 2); }
 
-// A chunk's g carried out of its start, from zero, and the product of its decays.
-template <typename T, int NS>
+// A chunk's g carried out of its start, from zero, and the product of its
+// decays; eight steps at a time, as scan_forward.
+template <typename T, int NS, bool GATED>
 __global__ __launch_bounds__(64) void scan_backward_ends(ScanArgs a, GradArgs ga) {
+    constexpr int TT = 8;
     const Place p = place_of(a);
     float A2[NS], g[NS];
     load_rates<NS>(a, p.d, A2);
 #pragma unroll
     for (int n = 0; n < NS; ++n) g[n] = 0.0f;
     const float bias = a.bias ? a.bias[p.d] : 0.0f;
-    const T* dp = (const T*)a.dt.p + p.b * a.dt.b + p.d;
-    const T* op = (const T*)ga.dout.p + p.b * ga.dout.b + p.d;
-    const T* zp = a.z.p ? (const T*)a.z.p + p.b * a.z.b + p.d : nullptr;
-    const uniform_f32 bc = (uniform_f32)(uintptr_t)(a.bc + (int64_t)p.b * a.length * 2 * NS);
+    const int total = (int)(p.t1 - p.t0);
+    const T* dp = (const T*)a.dt.p + p.b * a.dt.b + (p.t1 - 1) * a.dt.t + p.base;
+    const T* op = (const T*)ga.dout.p + p.b * ga.dout.b + (p.t1 - 1) * ga.dout.t + p.base;
+    const T* zp = GATED ? (const T*)a.z.p + p.b * a.z.b + (p.t1 - 1) * a.z.t + p.base : nullptr;
+    const uniform_f32 bc = (uniform_f32)(uintptr_t)(a.bc + ((int64_t)p.b * a.length + p.t0) * 2 * NS + NS);   // C
     float sum = 0.0f;
     bool cut = false;
-    uint64_t starts = 0;
-    int64_t from = p.t1;   // first step that `starts` speaks of
-    for (int64_t t = p.t1 - 1; t >= p.t0; --t) {
-        if (a.resets && t < from) {
-            from = p.t0 + (t - p.t0) / 64 * 64;
-            starts = resets_at(a, p.b, from, p.t1);
+    T dr[TT], orr[TT], zr[TT];
+    int left = total;   // steps not yet fetched
+    auto fetch = [&]() {
+#pragma unroll
+        for (int i = 0; i < TT; ++i) {
+            dr[i] = dp[p.lane];
+            orr[i] = op[p.lane];
+            if (GATED) zr[i] = zp[p.lane];
+            --left;
+            dp -= left > 0 ? a.dt.t : 0;   // past the start the first one again
+            op -= left > 0 ? ga.dout.t : 0;
+            if (GATED) zp -= left > 0 ? a.z.t : 0;
         }
-        float dl = (float)dp[t * a.dt.t] + bias;
-        if (a.softplus) dl = softplus(dl);
-        float dy = (float)op[t * ga.dout.t];
-        if (zp) {
-            const float z = (float)zp[t * a.z.t];
-            dy *= z * sigmoid(z);
+    };
+    struct C {
+        float v[NS];
+        __device__ __forceinline__ explicit C(uniform_f32 row) {
+#pragma unroll
+            for (int n = 0; n < NS; ++n) v[n] = row[n];
         }
-        const uniform_f32 row = bc + t * 2 * NS + NS;
+    };
+    auto step = [&](float dl, float dy, const C& row) {
         sum += dl;
 #pragma unroll
-        for (int n = 0; n < NS; ++n) g[n] = __builtin_fmaf(dy, row[n], g[n]) * exp2_fast(dl * A2[n]);
-        if (starts >> (t - from) & 1) {
-            cut = true;
+        for (int n = 0; n < NS; ++n) g[n] = __builtin_fmaf(dy, row.v[n], g[n]) * exp2_fast(dl * A2[n]);
+    };
+    fetch();
+#pragma unroll 1
+    for (int t = total - 1; t >= 0; t -= TT) {   // steps t, t - 1, ..
+        float dl[TT], dy[TT];
 #pragma unroll
-            for (int n = 0; n < NS; ++n) g[n] = 0.0f;
+        for (int i = 0; i < TT; ++i) {
+            dl[i] = (float)dr[i] + bias;
+            dy[i] = (float)orr[i];
+            if (GATED) {
+                const float z = (float)zr[i];
+                dy[i] *= z * sigmoid(z);
+            }
+        }
+        if (a.softplus) {
+#pragma unroll
+            for (int i = 0; i < TT; ++i) dl[i] = softplus(dl[i]);
+        }
+        if (t >= TT) fetch();
+        uint64_t cuts = 0;   // bit i: does a sequence begin at t - i?
+        if (a.resets) {
+            const int lane = threadIdx.x;
+            const bool r = lane < TT && lane <= t && a.resets[p.b * a.resets_b + (p.t0 + t - lane) * a.resets_t] != 0;
+            cuts = __ballot(r);
+        }
+        if (t >= TT - 1 && cuts == 0) {
+            C row(bc + (int64_t)t * 2 * NS);
+#pragma unroll
+            for (int i = 0; i < TT; ++i) {
+                const C next(bc + (int64_t)(t - i - 1 >= 0 ? t - i - 1 : 0) * 2 * NS);
+                __builtin_amdgcn_sched_barrier(0);   // sent off here, waited for a step later
+                step(dl[i], dy[i], row);
+                row = next;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < TT; ++i) {
+                if (i > t) break;
+                step(dl[i], dy[i], C(bc + (int64_t)(t - i) * 2 * NS));
+                if (cuts >> i & 1) {
+                    cut = true;
+#pragma unroll
+                    for (int n = 0; n < NS; ++n) g[n] = 0.0f;
+                }
+            }
         }
     }
     if (!p.live) return;
@@ -537,10 +591,13 @@ __global__ __launch_bounds__(64, 2) void scan_backward(ScanArgs a, GradArgs ga) 
         // forwards through the tile: w = what each step keeps of its past.
         // Steps past the end are of nothing: D = 0, x = 0, dy = 0.
         const uniform_f32 rows = bc + t * 2 * NS;
+        BC<NS> now(rows);
 #pragma unroll
         for (int i = 0; i < TT; ++i) {
             const bool in = !SLOW || i < steps;
-            const uniform_f32 row = rows + (in ? i : 0) * 2 * NS;
+            const float(&row)[2 * NS] = now.v;
+            const BC<NS> next(rows + (i + 1 < TT && (!SLOW || i + 1 < steps) ? i + 1 : 0) * 2 * NS);
+            if (kAhead<NS>) __builtin_amdgcn_sched_barrier(0);   // sent off here, waited for a step later
             if (SLOW && !in) dl[i] = 0.0f;
             x[i] = in ? (float)xr[i] : 0.0f;
             const float dout = in ? (float)orr[i] : 0.0f;
@@ -568,6 +625,7 @@ __global__ __launch_bounds__(64, 2) void scan_backward(ScanArgs a, GradArgs ga) 
                 T* row_dz = dzp + (t + i) * a.channels;
                 if (in) row_dz[p.lane] = (T)(dout * (y0 + y1) * s * __builtin_fmaf(z, 1.0f - s, 1.0f));
             }
+            now = next;
         }
         float r[G];
         // B and C are loaded anew: held since the walk forwards, a tile's rows
@@ -575,10 +633,13 @@ __global__ __launch_bounds__(64, 2) void scan_backward(ScanArgs a, GradArgs ga) 
         uint64_t again = (uint64_t)(uintptr_t)rows;
         asm volatile("" : "+s"(again));
         const uniform_f32 rows2 = (uniform_f32)(uintptr_t)again;
+        now = BC<NS>(rows2 + (!SLOW || TT - 1 < steps ? TT - 1 : 0) * 2 * NS);
 #pragma unroll
         for (int i = TT - 1; i >= 0; --i) {
             const bool in = !SLOW || i < steps;
-            const uniform_f32 row = rows2 + (in ? i : 0) * 2 * NS;
+            const float(&row)[2 * NS] = now.v;
+            const BC<NS> next(rows2 + (i > 0 && (!SLOW || i - 1 < steps) ? i - 1 : 0) * 2 * NS);
+            if (kAhead<NS>) __builtin_amdgcn_sched_barrier(0);
             const float u = dl[i] * x[i];
             const float u_sum = p.live ? u : 0.0f, dy_sum = p.live ? dy[i] : 0.0f;
             float gb = 0.0f, ga_ = 0.0f;
@@ -612,6 +673,7 @@ __global__ __launch_bounds__(64, 2) void scan_backward(ScanArgs a, GradArgs ga) 
                 float* row_part = part + (t + i) * 2 * NS;
                 if (!SLOW || i + k / (2 * NS) < steps) row_part[k] = s;
             }
+            now = next;
         }
     };
 
@@ -974,7 +1036,10 @@ SDFR_API int32_t sdfr_scan_grad(const SdfrScan* s, const SdfrScanGrad* g, void* 
             constexpr int NS = decltype(ns)::value;
             launch_pack<T, NS>(s, a, st);
             if (p.chunks > 1) {
-                scan_backward_ends<T, NS><<<(unsigned)grid, 64, 0, st>>>(a, ga);
+                if (s->z)
+                    scan_backward_ends<T, NS, true><<<(unsigned)grid, 64, 0, st>>>(a, ga);
+                else
+                    scan_backward_ends<T, NS, false><<<(unsigned)grid, 64, 0, st>>>(a, ga);
                 scan_join<true><<<(unsigned)(((int64_t)s->batch * NS * s->channels + 255) / 256), 256, 0, st>>>(
                     a.ends, a.prods, g->dstate_out, s->batch, p.chunks, NS, s->channels, s->states);
             }
