@@ -13,9 +13,11 @@
 //   dx[t] = sum_j w[width-1-j] dpre[t+j]     (j that see t)
 //   dw[width-1-j] = sum_t dpre[t] x[t-j],    dbias = sum_t dpre[t]
 //
-// A thread takes 16 bytes of channels of one sequence and walks a run of
-// steps with the window in registers, so inputs are read once but for the
-// run's first width-1 rows.
+// A thread takes four channels of one sequence and walks a run of steps with
+// the window in registers, so inputs are read once but for the run's first
+// width-1 rows; the next four steps' rows are on their way meanwhile. Where a
+// sequence begins the window is emptied, so a step only looks for a beginning
+// at itself.
 
 #include "recurrent.h"
 
@@ -24,7 +26,10 @@ namespace {
 using namespace rec;
 
 constexpr int kRun = 16;       // steps a thread walks
+constexpr int kTile = 4;       // steps whose rows are loaded together
 constexpr int kMaxWidth = 8;
+constexpr int V = 4;           // channels a thread
+constexpr int kThreads = 256;
 
 struct ConvArgs {
     const void* x;
@@ -38,7 +43,11 @@ struct ConvArgs {
     void* state_out;              // dense, or null
     int64_t length;
     int batch, channels, width, silu;
-    int vecs, runs;               // channel vectors a row, runs a sequence
+    int vecs;                     // channel vectors a row
+    int lanes;                    // threads side by side on a row: a power of two, up to 64
+    int across;                   // groups of lanes on a row
+    int runs;                     // of a sequence
+    int64_t jobs;                 // batch * runs
 };
 
 struct ConvGradArgs {
@@ -49,27 +58,30 @@ struct ConvGradArgs {
     void* dstate;                 // dense like state, or null
     float* sums;                  // (partial rows, width + 1, channels)
     int rows;                     // partial rows
-    int64_t jobs;                 // batch * runs
 };
 
-// V channels of a row. Rows of odd sizes or strides start anywhere: the loads
-// go by bytes (global memory takes any address), and a row's last vector by
-// elements.
-template <typename T, int V>
-__device__ inline void load_row(const T* p, int n, float (&v)[V]) {
+// Four channels as they lie in memory. Rows of odd sizes or strides start
+// anywhere: the loads go by bytes (global memory takes any address), and a
+// row's last vector by elements.
+template <typename T>
+struct Raw {
+    T r[V];
+};
+
+template <typename T>
+__device__ __forceinline__ Raw<T> load_raw(const T* p, int n) {
+    Raw<T> v;
     if (n >= V) {
-        T r[V];
-        __builtin_memcpy(r, p, sizeof r);
-#pragma unroll
-        for (int i = 0; i < V; ++i) v[i] = (float)r[i];
+        __builtin_memcpy(v.r, p, sizeof v.r);
     } else {
 #pragma unroll
-        for (int i = 0; i < V; ++i) v[i] = i < n ? (float)p[i] : 0.0f;
+        for (int i = 0; i < V; ++i) v.r[i] = i < n ? p[i] : (T)0.0f;
     }
+    return v;
 }
 
-template <typename T, int V>
-__device__ inline void store_row(T* p, int n, const float (&v)[V]) {
+template <typename T>
+__device__ __forceinline__ void store_row(T* p, int n, const float (&v)[V]) {
     if (n >= V) {
         T r[V];
 #pragma unroll
@@ -82,232 +94,393 @@ __device__ inline void store_row(T* p, int n, const float (&v)[V]) {
     }
 }
 
-// Row t of the input, t >= -(width-1): before the first step, of the state.
-template <typename T, int V>
-__device__ inline void load_input(const ConvArgs& a, int b, int64_t t, int c, int n, float (&v)[V]) {
-    if (t >= 0) {
-        load_row<T, V>((const T*)a.x + b * a.x_b + t * a.x_t + c, n, v);
-    } else if (a.state && t >= -(int64_t)(a.width - 1)) {
-        load_row<T, V>((const T*)a.state + ((int64_t)b * (a.width - 1) + (a.width - 1 + t)) * a.channels + c, n, v);
-    } else {
+template <typename T>
+__device__ __forceinline__ void widen(const Raw<T>& r, float (&v)[V]) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) v[i] = 0.0f;
-    }
+    for (int i = 0; i < V; ++i) v[i] = (float)r.r[i];
 }
 
-__device__ inline bool begins(const ConvArgs& a, int b, int64_t t) {
-    return a.resets && t >= 0 && t < a.length && a.resets[b * a.resets_b + t * a.resets_t] != 0;
-}
-
-// How many of the steps before t the window at t sees: up to width - 1, fewer
-// where a sequence begins in between.
-__device__ inline int sight_at(const ConvArgs& a, int b, int64_t t) {
-    int s = 0;
-    while (s < a.width - 1 && !begins(a, b, t - s)) ++s;
-    return s;
-}
-
-__device__ inline int next_sight(const ConvArgs& a, int b, int64_t t, int sight) {
-    return begins(a, b, t) ? 0 : sight < a.width - 1 ? sight + 1 : a.width - 1;
-}
-
-template <int V>
-__device__ inline void shift_in(float (&win)[V], const float (&v)[V]) {
+__device__ __forceinline__ void empty(float (&v)[V]) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) win[i] = v[i];
+    for (int i = 0; i < V; ++i) v[i] = 0.0f;
 }
 
-template <int W, int V>
-__device__ inline void load_weights(const ConvArgs& a, int c, int n, float (&w)[W][V], float (&bias)[V]) {
+// Row t < 0 of the input: of the state, or zeros.
+template <typename T>
+__device__ __forceinline__ void load_past(const ConvArgs& a, int b, int64_t t, int c, int n, float (&v)[V]) {
+    if (a.state && t >= -(int64_t)(a.width - 1))
+        widen(load_raw((const T*)a.state + ((int64_t)b * (a.width - 1) + (a.width - 1 + t)) * a.channels + c, n), v);
+    else
+        empty(v);
+}
+
+// w[j]: the weights of the input j steps back. W is the width, or (8) at least it.
+template <int W>
+__device__ __forceinline__ void load_weights(const ConvArgs& a, int c, int n, float (&w)[W][V], float (&bias)[V]) {
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-        bias[i] = i < n && a.bias ? a.bias[c + i] : 0.0f;
+        const int ch = i < n ? c + i : c;
+        bias[i] = a.bias ? a.bias[ch] : 0.0f;
+        if constexpr (W < kMaxWidth) {
+            float r[W];
+            __builtin_memcpy(r, a.weight + (int64_t)ch * W, sizeof r);
 #pragma unroll
-        for (int j = 0; j < W; ++j)   // w[j]: the weight of the input j steps back
-            w[j][i] = i < n && j < a.width ? a.weight[(int64_t)(c + i) * a.width + a.width - 1 - j] : 0.0f;
+            for (int j = 0; j < W; ++j) w[j][i] = r[W - 1 - j];
+        } else {
+#pragma unroll
+            for (int j = 0; j < W; ++j) {
+                const float r = a.weight[(int64_t)ch * a.width + (j < a.width ? a.width - 1 - j : 0)];
+                w[j][i] = j < a.width ? r : 0.0f;
+            }
+        }
     }
 }
 
-// pre at a step whose window is win[0] (now) .. win[W-1]; the first `sight`
-// steps back are seen. What is not seen is not multiplied: it may be anything.
-template <int W, int V>
-__device__ inline void convolve(const float (&win)[W][V], const float (&w)[W][V], const float (&bias)[V], int sight,
-                                float (&pre)[V]) {
+// Which of COUNT steps from t on a sequence begins at; before the first step
+// and past the end none does. All the loads go out together.
+template <int COUNT>
+__device__ __forceinline__ unsigned beginnings(const ConvArgs& a, int b, int64_t t) {
+    unsigned bits = 0;
+    if (a.resets) {
+        const uint8_t* r = a.resets + b * a.resets_b;
 #pragma unroll
-    for (int i = 0; i < V; ++i) pre[i] = __builtin_fmaf(w[0][i], win[0][i], bias[i]);
-#pragma unroll
-    for (int j = 1; j < W; ++j)
-        if (j <= sight) {
-#pragma unroll
-            for (int i = 0; i < V; ++i) pre[i] = __builtin_fmaf(w[j][i], win[j][i], pre[i]);
+        for (int i = 0; i < COUNT; ++i) {
+            const int64_t k = t + i;
+            const bool in = k >= 0 && k < a.length;
+            bits |= (unsigned)(in && r[(in ? k : 0) * a.resets_t] != 0) << i;
         }
+    }
+    return bits;
 }
 
-template <typename T, int W, int V>
-__global__ __launch_bounds__(256) void conv_forward(ConvArgs a) {
-    const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    const int64_t job = id / a.vecs;
-    if (job >= (int64_t)a.batch * a.runs) return;
-    const int c = (int)(id % a.vecs) * V, n = a.channels - c;
+// pre at a step whose window is win[0] (now) .. win[W-1]
+template <int W>
+__device__ __forceinline__ void convolve(const float (&win)[W][V], const float (&w)[W][V], const float (&bias)[V],
+                                         float (&pre)[V]) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        pre[i] = bias[i];
+#pragma unroll
+        for (int j = W - 1; j >= 0; --j) pre[i] = __builtin_fmaf(w[j][i], win[j][i], pre[i]);
+    }
+}
+
+// The window before step t0: the inputs 1 .. width-1 steps back, those that the
+// step before would still see (the step itself looks for its own beginning).
+template <typename T, int W>
+__device__ __forceinline__ void load_window(const ConvArgs& a, int b, int64_t t0, int c, int n, float (&win)[W][V]) {
+    const T* xp = (const T*)a.x + b * a.x_b + c;
+    const unsigned cuts = t0 > 0 ? beginnings<W - 1>(a, b, t0 - (W - 1)) : 0;   // bit i: at t0 - (W-1) + i
+    bool seen = true;
+#pragma unroll
+    for (int j = 1; j < W; ++j) {   // win[j-1] is shifted to win[j] at the first step
+        if (j >= a.width || !seen)
+            empty(win[j - 1]);
+        else if (t0 - j >= 0)
+            widen(load_raw(xp + (t0 - j) * a.x_t, n), win[j - 1]);
+        else
+            load_past<T>(a, b, t0 - j, c, n, win[j - 1]);
+        if (cuts >> (W - 1 - j) & 1) seen = false;   // what lies before t0 - j
+    }
+    empty(win[W - 1]);
+}
+
+// How many steps back a window reaches.
+template <int W>
+__device__ __forceinline__ int reach_of(const ConvArgs& a) {
+    return W < kMaxWidth ? W - 1 : a.width - 1;
+}
+
+template <int W>
+__device__ __forceinline__ void shift(float (&win)[W][V], int reach) {
+#pragma unroll
+    for (int j = W - 1; j > 0; --j)
+#pragma unroll
+        for (int i = 0; i < V; ++i) win[j][i] = W < kMaxWidth || j <= reach ? win[j - 1][i] : 0.0f;
+}
+
+// This thread's channels and job; false if it has none.
+__device__ __forceinline__ bool place(const ConvArgs& a, int64_t jobs, int* c, int* n, int64_t* job) {
+    const int lane = threadIdx.x & (a.lanes - 1);
+    const int vec = (int)(blockIdx.x % a.across) * a.lanes + lane;
+    *job = blockIdx.x / a.across * (int64_t)(kThreads / a.lanes) + threadIdx.x / a.lanes;
+    *c = vec * V;
+    *n = a.channels - vec * V;
+    return vec < a.vecs && *job < jobs;
+}
+
+template <typename T, int W>
+__global__ __launch_bounds__(kThreads) void conv_forward(ConvArgs a) {
+    int c, n;
+    int64_t job;
+    if (!place(a, a.jobs, &c, &n, &job)) return;
     const int b = (int)(job / a.runs);
     const int64_t t0 = job % a.runs * kRun;
-    const int64_t t1 = t0 + kRun < a.length ? t0 + kRun : a.length;
+    const int steps = a.length - t0 < kRun ? (int)(a.length - t0) : kRun;
+    const T* xp = (const T*)a.x + b * a.x_b + t0 * a.x_t + c;
+    T* yp = (T*)a.y + b * a.y_b + t0 * a.y_t + c;
+    Raw<T> ahead[kTile];
+    auto fetch = [&](int s) {
+#pragma unroll
+        for (int q = 0; q < kTile; ++q) ahead[q] = load_raw(xp + (s + q < steps ? s + q : steps - 1) * a.x_t, n);
+    };
+    fetch(0);
+    const unsigned cuts = beginnings<kRun>(a, b, t0);
     float w[W][V], bias[V], win[W][V];
-    load_weights<W, V>(a, c, n, w, bias);
+    load_weights<W>(a, c, n, w, bias);
+    load_window<T, W>(a, b, t0, c, n, win);
+    for (int s = 0; s < steps; s += kTile) {
+        Raw<T> now[kTile];
 #pragma unroll
-    for (int j = 1; j < W; ++j) load_input<T, V>(a, b, t0 - j, c, n, win[j - 1]);   // shifted at the first step
-    int sight = a.resets ? sight_at(a, b, t0 - 1) : a.width - 1;
-    T* yp = (T*)a.y + b * a.y_b + c;
-    for (int64_t t = t0; t < t1; ++t) {
+        for (int q = 0; q < kTile; ++q) now[q] = ahead[q];
+        if (s + kTile < steps) fetch(s + kTile);
 #pragma unroll
-        for (int j = W - 1; j > 0; --j) shift_in<V>(win[j], win[j - 1]);
-        load_input<T, V>(a, b, t, c, n, win[0]);
-        sight = next_sight(a, b, t, sight);
-        float pre[V];
-        convolve<W, V>(win, w, bias, sight, pre);
+        for (int q = 0; q < kTile; ++q) {
+            if (s + q >= steps) break;
+            shift(win, reach_of<W>(a));
+            widen(now[q], win[0]);
+            if (cuts >> (s + q) & 1) {
+#pragma unroll
+                for (int j = 1; j < W; ++j) empty(win[j]);
+            }
+            float pre[V];
+            convolve(win, w, bias, pre);
+            if (a.silu) {
+#pragma unroll
+                for (int i = 0; i < V; ++i) pre[i] *= sigmoid(pre[i]);
+            }
+            store_row(yp + (s + q) * a.y_t, n, pre);
+        }
+    }
+    if (a.state_out && t0 + steps == a.length) {
+        // the window the next call starts from
+        T* so = (T*)a.state_out + (int64_t)b * (a.width - 1) * a.channels + c;
+#pragma unroll
+        for (int j = 0; j < W - 1; ++j)
+            if (j < a.width - 1) store_row(so + (int64_t)(a.width - 2 - j) * a.channels, n, win[j]);
+    }
+}
+
+// ---- a single step -------------------------------------------------------------
+// What it moves is the window; the weights, as many bytes again, are read once
+// for kRows sequences.
+constexpr int kRows = 4;
+
+template <typename T, int W>
+__global__ __launch_bounds__(kThreads) void conv_step(ConvArgs a) {
+    int c, n;
+    int64_t group;
+    if (!place(a, (a.batch + kRows - 1) / kRows, &c, &n, &group)) return;
+    float w[W][V], bias[V];
+    load_weights<W>(a, c, n, w, bias);
+    Raw<T> x[kRows], past[kRows][W];
+    bool cut[kRows];
+    const T* sp = (const T*)a.state;
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+        const int64_t b = group * kRows + r < a.batch ? group * kRows + r : a.batch - 1;
+        x[r] = load_raw((const T*)a.x + b * a.x_b + c, n);
+        cut[r] = a.resets && a.resets[b * a.resets_b] != 0;
+#pragma unroll
+        for (int j = 1; j < W; ++j)
+            if (sp && j < a.width) past[r][j] = load_raw(sp + (b * (a.width - 1) + a.width - 1 - j) * a.channels + c, n);
+    }
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+        const int64_t b = group * kRows + r;
+        if (b >= a.batch) break;
+        float win[W][V], pre[V];
+        widen(x[r], win[0]);
+#pragma unroll
+        for (int j = 1; j < W; ++j) {
+            if (!sp || j >= a.width || cut[r])
+                empty(win[j]);
+            else
+                widen(past[r][j], win[j]);
+        }
+        convolve(win, w, bias, pre);
         if (a.silu) {
 #pragma unroll
             for (int i = 0; i < V; ++i) pre[i] *= sigmoid(pre[i]);
         }
-        store_row<T, V>(yp + t * a.y_t, n, pre);
-    }
-    if (a.state_out && t1 == a.length) {
-        // the window the next call starts from; what it must not see is cleared
-        const float none[V] = {};
-        T* so = (T*)a.state_out + (int64_t)b * (a.width - 1) * a.channels + c;
+        store_row((T*)a.y + b * a.y_b + c, n, pre);
+        if (a.state_out) {
+            T* so = (T*)a.state_out + b * (a.width - 1) * a.channels + c;
 #pragma unroll
-        for (int j = 0; j < W - 1; ++j)
-            if (j < a.width - 1)
-                store_row<T, V>(so + (int64_t)(a.width - 2 - j) * a.channels, n, j <= sight ? win[j] : none);
+            for (int j = 0; j < W - 1; ++j)
+                if (j < a.width - 1) store_row(so + (int64_t)(a.width - 2 - j) * a.channels, n, win[j]);
+        }
     }
 }
 
 // A thread walks the runs of its share one after another with its sums of dw
-// and dbias in registers. Within a run it goes W - 1 steps past the end, whose
-// dpre the run's last inputs get their gradients from.
-template <typename T, int W, int V>
-__global__ __launch_bounds__(256) void conv_backward(ConvArgs a, ConvGradArgs g) {
-    const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    const int64_t share = id / a.vecs;
-    if (share >= g.rows) return;
-    const int c = (int)(id % a.vecs) * V, n = a.channels - c;
+// and dbias in registers; a workgroup adds up what its shares have. Within a
+// run it goes W - 1 steps past the end, whose dpre the run's last inputs get
+// their gradients from.
+template <typename T, int W>
+__global__ __launch_bounds__(kThreads) void conv_backward(ConvArgs a, ConvGradArgs g) {
+    constexpr int STEPS = kRun + W - 1;
+    __shared__ float lds[kThreads][V + 1];
+    int c, n;
+    int64_t share;
+    const int64_t shares = (int64_t)g.rows * (kThreads / a.lanes);
+    const bool any = place(a, shares, &c, &n, &share);
     float w[W][V], bias[V], dw[W][V], db[V];
-    load_weights<W, V>(a, c, n, w, bias);
+    empty(db);
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-        db[i] = 0.0f;
-#pragma unroll
-        for (int j = 0; j < W; ++j) dw[j][i] = 0.0f;
-    }
-    for (int64_t job = share; job < g.jobs; job += g.rows) {
+    for (int j = 0; j < W; ++j) empty(dw[j]);
+    if (any) load_weights<W>(a, c, n, w, bias);
+    for (int64_t job = any ? share : a.jobs; job < a.jobs; job += shares) {
         const int b = (int)(job / a.runs);
         const int64_t t0 = job % a.runs * kRun;
-        const int64_t t1 = t0 + kRun < a.length ? t0 + kRun : a.length;
-        // steps t0 .. end-1 have a dpre; the run owns the gradients of inputs
-        // t0 .. t1-1, the first one those of the state too
-        const int64_t end = t1 + W - 1 < a.length ? t1 + W - 1 : a.length;
-        float win[W][V], acc[W][V];   // acc[j]: gradient of the input j steps back, so far
+        const int own = a.length - t0 < kRun ? (int)(a.length - t0) : kRun;
+        // steps t0 .. t0+steps-1 have a dpre; the run owns the gradients of
+        // inputs t0 .. t0+own-1, the first run those of the state too
+        const int steps = a.length - t0 < own + W - 1 ? (int)(a.length - t0) : own + W - 1;
+        const T* xp = (const T*)a.x + b * a.x_b + t0 * a.x_t + c;
+        const T* dyp = (const T*)g.dy + b * g.dy_b + t0 * g.dy_t + c;
+        T* dxp = (T*)g.dx + ((int64_t)b * a.length + t0) * a.channels + c;
+        Raw<T> xa[kTile], da[kTile];
+        auto fetch = [&](int s) {
 #pragma unroll
-        for (int j = 1; j < W; ++j) load_input<T, V>(a, b, t0 - j, c, n, win[j - 1]);
-#pragma unroll
-        for (int j = 0; j < W; ++j)
-#pragma unroll
-            for (int i = 0; i < V; ++i) acc[j][i] = 0.0f;
-        int sight = a.resets ? sight_at(a, b, t0 - 1) : a.width - 1;
-        const T* dyp = (const T*)g.dy + b * g.dy_b + c;
-        auto put = [&](int64_t t, float (&v)[V]) {   // the gradient of input t is whole
-            if (t >= t0 && t < t1) {
-                store_row<T, V>((T*)g.dx + ((int64_t)b * a.length + t) * a.channels + c, n, v);
-            } else if (t0 == 0 && t < 0 && g.dstate && t >= -(int64_t)(a.width - 1)) {
-                store_row<T, V>((T*)g.dstate + ((int64_t)b * (a.width - 1) + a.width - 1 + t) * a.channels + c, n, v);
+            for (int q = 0; q < kTile; ++q) {
+                const int k = s + q < steps ? s + q : steps - 1;
+                xa[q] = load_raw(xp + k * a.x_t, n);
+                da[q] = load_raw(dyp + k * g.dy_t, n);
             }
         };
-        for (int64_t t = t0; t < end; ++t) {
+        fetch(0);
+        const unsigned cuts = beginnings<STEPS>(a, b, t0);
+        float win[W][V], acc[W][V];   // acc[j]: gradient of the input j steps back, so far
+        load_window<T, W>(a, b, t0, c, n, win);
 #pragma unroll
-            for (int j = W - 1; j > 0; --j) {
-                shift_in<V>(win[j], win[j - 1]);
-                shift_in<V>(acc[j], acc[j - 1]);
+        for (int j = 0; j < W; ++j) empty(acc[j]);
+        // how far back the step before sees; only the state's gradient and a
+        // beginning make it less than everything
+        const int reach = reach_of<W>(a);
+        int sight = reach;
+        if (t0 > 0 && a.resets) {
+            const unsigned past = beginnings<W - 1>(a, b, t0 - (W - 1));
+            const int s = past ? __clz(past << (32 - (W - 1))) : reach;
+            sight = s < reach ? s : reach;
+        }
+        auto put = [&](int t, float (&v)[V]) {   // the gradient of input t0 + t is whole
+            if (t >= 0 && t < own) {
+                store_row(dxp + (int64_t)t * a.channels, n, v);
+            } else if (t0 == 0 && t < 0 && g.dstate && t >= -(a.width - 1)) {
+                store_row((T*)g.dstate + ((int64_t)b * (a.width - 1) + a.width - 1 + t) * a.channels + c, n, v);
             }
+        };
+        for (int s = 0; s < steps; s += kTile) {
+            Raw<T> xn[kTile], dn[kTile];
 #pragma unroll
-            for (int i = 0; i < V; ++i) acc[0][i] = 0.0f;
-            load_input<T, V>(a, b, t, c, n, win[0]);
-            sight = next_sight(a, b, t, sight);
-            float d[V];
-            load_row<T, V>(dyp + t * g.dy_t, n, d);
-            if (a.silu) {
-                float pre[V];
-                convolve<W, V>(win, w, bias, sight, pre);
+            for (int q = 0; q < kTile; ++q) xn[q] = xa[q], dn[q] = da[q];
+            if (s + kTile < steps) fetch(s + kTile);
 #pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    const float s = sigmoid(pre[i]);
-                    d[i] *= s * __builtin_fmaf(pre[i], 1.0f - s, 1.0f);
+            for (int q = 0; q < kTile; ++q) {
+                const int t = s + q;
+                if (t >= steps) break;
+                shift(win, reach);
+                shift(acc, W);   // the gradients go on to where they are put
+                empty(acc[0]);
+                widen(xn[q], win[0]);
+                sight = sight < reach ? sight + 1 : reach;
+                if (cuts >> t & 1) {
+                    sight = 0;
+#pragma unroll
+                    for (int j = 1; j < W; ++j) empty(win[j]);
                 }
-            }
-            const bool own = t < t1;
-#pragma unroll
-            for (int j = 0; j < W; ++j)
-                if (j <= sight) {
+                float d[V];
+                widen(dn[q], d);
+                if (a.silu) {
+                    float pre[V];
+                    convolve(win, w, bias, pre);
 #pragma unroll
                     for (int i = 0; i < V; ++i) {
-                        acc[j][i] = __builtin_fmaf(w[j][i], d[i], acc[j][i]);
-                        if (own) dw[j][i] = __builtin_fmaf(d[i], win[j][i], dw[j][i]);
+                        const float s1 = sigmoid(pre[i]);
+                        d[i] *= s1 * __builtin_fmaf(pre[i], 1.0f - s1, 1.0f);
                     }
                 }
-            if (own) {
 #pragma unroll
-                for (int i = 0; i < V; ++i) db[i] += d[i];
+                for (int j = 0; j < W; ++j)
+                    if (j <= sight) {
+#pragma unroll
+                        for (int i = 0; i < V; ++i) acc[j][i] = __builtin_fmaf(w[j][i], d[i], acc[j][i]);
+                    }
+                if (t < own) {
+#pragma unroll
+                    for (int j = 0; j < W; ++j)
+#pragma unroll
+                        for (int i = 0; i < V; ++i) dw[j][i] = __builtin_fmaf(d[i], win[j][i], dw[j][i]);
+#pragma unroll
+                    for (int i = 0; i < V; ++i) db[i] += d[i];
+                }
+                put(t - (W - 1), acc[W - 1]);
             }
-            put(t - (W - 1), acc[W - 1]);
         }
-        // inputs whose later readers lie past the sequence's end; the window
-        // handed on holds the last ones
+        if (t0 + steps == a.length) {
+            // inputs whose later readers lie past the sequence's end; the
+            // window handed on holds the last ones
 #pragma unroll
-        for (int j = W - 2; j >= 0; --j) {
-            const int64_t t = end - 1 - j;
-            if (end == a.length && g.dstate_out && j < a.width - 1 && j <= sight) {
-                float v[V];
-                load_row<T, V>((const T*)g.dstate_out + ((int64_t)b * (a.width - 1) + a.width - 2 - j) * a.channels + c,
-                               n, v);
+            for (int j = W - 2; j >= 0; --j) {
+                if (g.dstate_out && j < a.width - 1 && j <= sight) {
+                    float v[V];
+                    widen(load_raw((const T*)g.dstate_out +
+                                       ((int64_t)b * (a.width - 1) + a.width - 2 - j) * a.channels + c, n), v);
 #pragma unroll
-                for (int i = 0; i < V; ++i) acc[j][i] += v[i];
+                    for (int i = 0; i < V; ++i) acc[j][i] += v[i];
+                }
+                put(steps - 1 - j, acc[j]);
             }
-            if (end == a.length) put(t, acc[j]);
         }
     }
-    float* s = g.sums + share * (a.width + 1) * a.channels + c;
+    // the workgroup's shares, one column of sums after another
+    const int row = (int)(blockIdx.x / a.across);
+    float* out = g.sums + (int64_t)row * (a.width + 1) * a.channels;
+    const int groups = kThreads / a.lanes;
 #pragma unroll
-    for (int j = 0; j < W; ++j)
-        if (j < a.width) {
+    for (int j = 0; j <= W; ++j) {
+        if (j < W && j >= a.width) continue;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < V; ++i) lds[threadIdx.x][i] = j < W ? dw[j < W ? j : 0][i] : db[i];
+        __syncthreads();
+        if ((int)threadIdx.x < a.lanes) {
+            float s[V];
+            empty(s);
+            for (int k = 0; k < groups; ++k)
+#pragma unroll
+                for (int i = 0; i < V; ++i) s[i] += lds[threadIdx.x + k * a.lanes][i];
 #pragma unroll
             for (int i = 0; i < V; ++i)
-                if (i < n) s[(int64_t)j * a.channels + i] = dw[j][i];
+                if (any && i < n) out[(int64_t)(j < W ? j : a.width) * a.channels + c + i] = s[i];
         }
-#pragma unroll
-    for (int i = 0; i < V; ++i)
-        if (i < n) s[(int64_t)a.width * a.channels + i] = db[i];
+    }
 }
 
-// dw and dbias from the shares' sums, always in the same order.
+// dw and dbias from the workgroups' sums, always in the same order: 32 columns
+// a block, 32 shares of the rows.
 __global__ __launch_bounds__(1024) void conv_sums(const float* __restrict__ sums, float* dw, float* dbias, int rows,
                                                   int width, int channels) {
-    __shared__ float lds[16][64];
+    __shared__ float lds[32][33];
     const int64_t cols = (int64_t)(width + 1) * channels;
-    const int64_t c = (int64_t)blockIdx.x * 64 + threadIdx.x;
+    const int64_t c = (int64_t)blockIdx.x * 32 + threadIdx.x;
     float s = 0.0f;
-    if (c < cols)
-        for (int64_t r = threadIdx.y; r < rows; r += 16) s += sums[r * cols + c];
+    if (c < cols) {
+#pragma unroll 4
+        for (int r = threadIdx.y; r < rows; r += 32) s += sums[r * cols + c];
+    }
     lds[threadIdx.y][threadIdx.x] = s;
     __syncthreads();
     if (threadIdx.y != 0 || c >= cols) return;
-    for (int j = 1; j < 16; ++j) s += lds[j][threadIdx.x];
+#pragma unroll
+    for (int j = 1; j < 32; ++j) s += lds[j][threadIdx.x];
     const int j = (int)(c / channels), d = (int)(c % channels);
     if (j < width)
         dw[(int64_t)d * width + width - 1 - j] = s;
     else if (dbias)
         dbias[d] = s;
 }
-
-int vec_of(int32_t dtype) { return dtype == SDFR_F32 ? 4 : 8; }
 
 int32_t check_conv(const char* fn, const SdfrConv* s) {
     g_rec_err[0] = '\0';
@@ -318,7 +491,7 @@ int32_t check_conv(const char* fn, const SdfrConv* s) {
     if (s->width < 1 || s->width > kMaxWidth)
         return rec_fail(-2, "%s: width must be 1 to %d (got %d)", fn, kMaxWidth, s->width);
     if (!rec_float(s->dtype)) return rec_fail(-3, "%s: dtype must be f32, f16 or bf16 (got %d)", fn, s->dtype);
-    const int64_t runs = (s->length + kRun - 1) / kRun, vecs = (s->channels + vec_of(s->dtype) - 1) / vec_of(s->dtype);
+    const int64_t runs = (s->length + kRun - 1) / kRun, vecs = (s->channels + V - 1) / V;
     if (s->channels > (1 << 24) || runs > 0x3fffffff || s->batch * runs > ((int64_t)1 << 38) / vecs)
         return rec_fail(-2, "%s: sizes too large", fn);
     if (!s->weight) return rec_fail(-1, "%s: null weight", fn);
@@ -348,23 +521,35 @@ ConvArgs conv_args(const SdfrConv* s) {
     a.channels = s->channels;
     a.width = s->width;
     a.silu = s->silu;
-    a.vecs = (s->channels + vec_of(s->dtype) - 1) / vec_of(s->dtype);
+    a.vecs = (s->channels + V - 1) / V;
+    a.lanes = 1;
+    while (a.lanes < 64 && a.lanes < a.vecs) a.lanes *= 2;
+    a.across = (a.vecs + a.lanes - 1) / a.lanes;
     a.runs = (int)((s->length + kRun - 1) / kRun);
+    a.jobs = (int64_t)a.batch * a.runs;
     return a;
 }
 
-// Partial sums the gradients of the parameters are gathered in: enough shares
-// to fill the machine, few enough that their sum is cheap.
+unsigned blocks_of(const ConvArgs& a, int64_t jobs) {
+    const int groups = kThreads / a.lanes;
+    return (unsigned)((jobs + groups - 1) / groups * a.across);
+}
+
+// Partial sums the gradients of the parameters are gathered in: one a
+// workgroup and, for it, as many shares as it has groups of lanes. Enough to
+// fill the machine, few enough that their sum is cheap.
 int conv_rows(const ConvArgs& a) {
-    const int64_t jobs = (int64_t)a.batch * a.runs;
-    const int64_t rows = (256 * 1024 + a.vecs - 1) / a.vecs;
-    return (int)(jobs < rows ? jobs : rows);
+    const int64_t groups = kThreads / a.lanes, whole = (a.jobs + groups - 1) / groups;
+    const int64_t rows = (2048 + a.across - 1) / a.across;
+    return (int)(whole < rows ? whole : rows);
 }
 
 template <class F>
 int32_t with_width(int width, F f) {
-    if (width <= 4) return f(std::integral_constant<int, 4>());
-    return f(std::integral_constant<int, 8>());
+    if (width == 2) return f(std::integral_constant<int, 2>());
+    if (width == 3) return f(std::integral_constant<int, 3>());
+    if (width == 4) return f(std::integral_constant<int, 4>());
+    return f(std::integral_constant<int, kMaxWidth>());
 }
 
 }  // namespace
@@ -379,11 +564,14 @@ SDFR_API int32_t sdfr_conv(const SdfrConv* s, void* stream) {
     if (s->length == 0) return rec_fail(-2, "%s: length must be positive", fn);
     hipStream_t st = (hipStream_t)stream;
     const ConvArgs a = conv_args(s);
-    const unsigned blocks = (unsigned)(((int64_t)a.batch * a.runs * a.vecs + 255) / 256);
     rec_typed(s->dtype, [&](auto v) {
         typedef decltype(v) T;
         return with_width(s->width, [&](auto w) {
-            conv_forward<T, decltype(w)::value, 16 / sizeof(T)><<<blocks, 256, 0, st>>>(a);
+            constexpr int W = decltype(w)::value;
+            if (s->length == 1)
+                conv_step<T, W><<<blocks_of(a, (a.batch + kRows - 1) / kRows), kThreads, 0, st>>>(a);
+            else
+                conv_forward<T, W><<<blocks_of(a, a.jobs), kThreads, 0, st>>>(a);
             return 0;
         });
     });
@@ -422,16 +610,14 @@ SDFR_API int32_t sdfr_conv_grad(const SdfrConv* s, const SdfrConvGrad* g, void* 
     ga.dstate = s->width > 1 ? g->dstate : nullptr;
     ga.sums = (float*)workspace;
     ga.rows = conv_rows(a);
-    ga.jobs = (int64_t)a.batch * a.runs;
-    const unsigned blocks = (unsigned)(((int64_t)ga.rows * a.vecs + 255) / 256);
     rec_typed(s->dtype, [&](auto v) {
         typedef decltype(v) T;
         return with_width(s->width, [&](auto w) {
-            conv_backward<T, decltype(w)::value, 16 / sizeof(T)><<<blocks, 256, 0, st>>>(a, ga);
+            conv_backward<T, decltype(w)::value><<<(unsigned)((int64_t)ga.rows * a.across), kThreads, 0, st>>>(a, ga);
             return 0;
         });
     });
-    conv_sums<<<(unsigned)(((int64_t)(s->width + 1) * s->channels + 63) / 64), dim3(64, 16), 0, st>>>(
+    conv_sums<<<(unsigned)(((int64_t)(s->width + 1) * s->channels + 31) / 32), dim3(32, 32), 0, st>>>(
         ga.sums, g->dweight, g->dbias, ga.rows, s->width, s->channels);
     return rec_launched(fn);
 }
