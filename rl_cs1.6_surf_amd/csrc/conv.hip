@@ -26,7 +26,8 @@ namespace {
 using namespace rec;
 
 constexpr int kRun = 16;       // steps a thread walks
-constexpr int kTile = 4;       // steps whose rows are loaded together
+// steps whose rows are loaded together: 64 bytes a thread and tensor
+template <typename T> constexpr int kTile = 16 / sizeof(T);
 constexpr int kMaxWidth = 8;
 constexpr int V = 4;           // channels a thread
 constexpr int kThreads = 256;
@@ -61,21 +62,42 @@ struct ConvGradArgs {
 };
 
 // Four channels as they lie in memory. Rows of odd sizes or strides start
-// anywhere: the loads go by bytes (global memory takes any address), and a
-// row's last vector by elements.
+// anywhere: the loads go by bytes (global memory takes any address). A row's
+// last vector, if it is not whole, is read as the row's last four channels and
+// moved down: no load is behind a branch, which would cost a wait each.
 template <typename T>
 struct Raw {
     T r[V];
 };
 
+// Where a thread's channels are.
+struct Chan {
+    int c, n;      // the first, and how many from there to the row's end
+    int back;      // how far before it the load starts
+    bool few;      // rows of less than four channels (uniform)
+};
+
 template <typename T>
-__device__ __forceinline__ Raw<T> load_raw(const T* p, int n) {
+__device__ __forceinline__ Raw<T> load_whole(const T* at) {
     Raw<T> v;
-    if (n >= V) {
-        __builtin_memcpy(v.r, p, sizeof v.r);
+    __builtin_memcpy(v.r, at, sizeof v.r);
+    return v;
+}
+
+template <typename T>
+__device__ __forceinline__ Raw<T> load_raw(const T* row, const Chan& ch) {
+    Raw<T> v;
+    if (!ch.few) {
+        __builtin_memcpy(v.r, row + (ch.c - ch.back), sizeof v.r);
+#pragma unroll
+        for (int k = 1; k < V; ++k)
+            if (ch.back >= k) {
+#pragma unroll
+                for (int i = 0; i + 1 < V; ++i) v.r[i] = v.r[i + 1];
+            }
     } else {
 #pragma unroll
-        for (int i = 0; i < V; ++i) v.r[i] = i < n ? p[i] : (T)0.0f;
+        for (int i = 0; i < V; ++i) v.r[i] = i < ch.n ? row[ch.c + i] : (T)0.0f;
     }
     return v;
 }
@@ -107,19 +129,19 @@ __device__ __forceinline__ void empty(float (&v)[V]) {
 
 // Row t < 0 of the input: of the state, or zeros.
 template <typename T>
-__device__ __forceinline__ void load_past(const ConvArgs& a, int b, int64_t t, int c, int n, float (&v)[V]) {
+__device__ __forceinline__ void load_past(const ConvArgs& a, int b, int64_t t, const Chan& ch, float (&v)[V]) {
     if (a.state && t >= -(int64_t)(a.width - 1))
-        widen(load_raw((const T*)a.state + ((int64_t)b * (a.width - 1) + (a.width - 1 + t)) * a.channels + c, n), v);
+        widen(load_raw((const T*)a.state + ((int64_t)b * (a.width - 1) + (a.width - 1 + t)) * a.channels, ch), v);
     else
         empty(v);
 }
 
 // w[j]: the weights of the input j steps back. W is the width, or (8) at least it.
 template <int W>
-__device__ __forceinline__ void load_weights(const ConvArgs& a, int c, int n, float (&w)[W][V], float (&bias)[V]) {
+__device__ __forceinline__ void load_weights(const ConvArgs& a, const Chan& at, float (&w)[W][V], float (&bias)[V]) {
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-        const int ch = i < n ? c + i : c;
+        const int ch = i < at.n ? at.c + i : at.c;
         bias[i] = a.bias ? a.bias[ch] : 0.0f;
         if constexpr (W < kMaxWidth) {
             float r[W];
@@ -137,18 +159,26 @@ __device__ __forceinline__ void load_weights(const ConvArgs& a, int c, int n, fl
 }
 
 // Which of COUNT steps from t on a sequence begins at; before the first step
-// and past the end none does. All the loads go out together.
+// and past the end none does. Where a wave is on one row its lanes load a step
+// each; else all the loads of a thread go out together.
 template <int COUNT>
 __device__ __forceinline__ unsigned beginnings(const ConvArgs& a, int b, int64_t t) {
     unsigned bits = 0;
-    if (a.resets) {
-        const uint8_t* r = a.resets + b * a.resets_b;
+    if (!a.resets) return bits;
+    const uint8_t* r = a.resets + b * a.resets_b;
+    if (a.lanes == 64) {
+        const int lane = threadIdx.x & 63;
+        const int64_t k = t + lane;
+        const bool in = lane < COUNT && k >= 0 && k < a.length;
+        // (in a wave that reaches past the row's end some lanes are gone, and their steps would not be loaded)
+        if (__ballot(true) == ~0ull) return (unsigned)__ballot(in && r[(in ? k : 0) * a.resets_t] != 0);
+    }
 #pragma unroll
-        for (int i = 0; i < COUNT; ++i) {
-            const int64_t k = t + i;
-            const bool in = k >= 0 && k < a.length;
-            bits |= (unsigned)(in && r[(in ? k : 0) * a.resets_t] != 0) << i;
-        }
+    for (int i = 0; i < COUNT; ++i) {
+        const int64_t k = t + i;
+        const bool in = k >= 0 && k < a.length;
+        const uint8_t v = r[(in ? k : 0) * a.resets_t];
+        bits |= (unsigned)(in & (v != 0)) << i;
     }
     return bits;
 }
@@ -168,18 +198,21 @@ __device__ __forceinline__ void convolve(const float (&win)[W][V], const float (
 // The window before step t0: the inputs 1 .. width-1 steps back, those that the
 // step before would still see (the step itself looks for its own beginning).
 template <typename T, int W>
-__device__ __forceinline__ void load_window(const ConvArgs& a, int b, int64_t t0, int c, int n, float (&win)[W][V]) {
-    const T* xp = (const T*)a.x + b * a.x_b + c;
+__device__ __forceinline__ void load_window(const ConvArgs& a, int b, int64_t t0, const Chan& ch, float (&win)[W][V]) {
+    const T* xp = (const T*)a.x + b * a.x_b;
     const unsigned cuts = t0 > 0 ? beginnings<W - 1>(a, b, t0 - (W - 1)) : 0;   // bit i: at t0 - (W-1) + i
     bool seen = true;
+    if (t0 >= W - 1) {
+#pragma unroll
+        for (int j = 1; j < W; ++j) widen(load_raw(xp + (t0 - j) * a.x_t, ch), win[j - 1]);
+    } else {   // the first run
+#pragma unroll
+        for (int j = 1; j < W; ++j) load_past<T>(a, b, t0 - j, ch, win[j - 1]);
+    }
 #pragma unroll
     for (int j = 1; j < W; ++j) {   // win[j-1] is shifted to win[j] at the first step
-        if (j >= a.width || !seen)
-            empty(win[j - 1]);
-        else if (t0 - j >= 0)
-            widen(load_raw(xp + (t0 - j) * a.x_t, n), win[j - 1]);
-        else
-            load_past<T>(a, b, t0 - j, c, n, win[j - 1]);
+#pragma unroll
+        for (int i = 0; i < V; ++i) win[j - 1][i] = j < a.width && seen ? win[j - 1][i] : 0.0f;
         if (cuts >> (W - 1 - j) & 1) seen = false;   // what lies before t0 - j
     }
     empty(win[W - 1]);
@@ -200,64 +233,93 @@ __device__ __forceinline__ void shift(float (&win)[W][V], int reach) {
 }
 
 // This thread's channels and job; false if it has none.
-__device__ __forceinline__ bool place(const ConvArgs& a, int64_t jobs, int* c, int* n, int64_t* job) {
+__device__ __forceinline__ bool place(const ConvArgs& a, int64_t jobs, Chan* ch, int64_t* job) {
     const int lane = threadIdx.x & (a.lanes - 1);
     const int vec = (int)(blockIdx.x % a.across) * a.lanes + lane;
     *job = blockIdx.x / a.across * (int64_t)(kThreads / a.lanes) + threadIdx.x / a.lanes;
-    *c = vec * V;
-    *n = a.channels - vec * V;
+    ch->c = vec * V;
+    ch->n = a.channels - vec * V;
+    ch->few = a.channels < V;
+    ch->back = ch->n < V && !ch->few ? V - ch->n : 0;
     return vec < a.vecs && *job < jobs;
 }
 
+// Whole runs without a beginning, as nearly all are, go without a question a
+// step and with the next rows on their way; the others step by step.
 template <typename T, int W>
 __global__ __launch_bounds__(kThreads) void conv_forward(ConvArgs a) {
-    int c, n;
+    constexpr int TT = kTile<T>;
+    Chan ch;
     int64_t job;
-    if (!place(a, a.jobs, &c, &n, &job)) return;
+    if (!place(a, a.jobs, &ch, &job)) return;
     const int b = (int)(job / a.runs);
     const int64_t t0 = job % a.runs * kRun;
     const int steps = a.length - t0 < kRun ? (int)(a.length - t0) : kRun;
-    const T* xp = (const T*)a.x + b * a.x_b + t0 * a.x_t + c;
-    T* yp = (T*)a.y + b * a.y_b + t0 * a.y_t + c;
-    Raw<T> ahead[kTile];
-    auto fetch = [&](int s) {
-#pragma unroll
-        for (int q = 0; q < kTile; ++q) ahead[q] = load_raw(xp + (s + q < steps ? s + q : steps - 1) * a.x_t, n);
-    };
-    fetch(0);
+    const T* xp = (const T*)a.x + b * a.x_b + t0 * a.x_t;
+    T* yp = (T*)a.y + b * a.y_b + t0 * a.y_t + ch.c;
     const unsigned cuts = beginnings<kRun>(a, b, t0);
+    const int reach = reach_of<W>(a);
     float w[W][V], bias[V], win[W][V];
-    load_weights<W>(a, c, n, w, bias);
-    load_window<T, W>(a, b, t0, c, n, win);
-    for (int s = 0; s < steps; s += kTile) {
-        Raw<T> now[kTile];
+    auto step = [&](const Raw<T>& row, bool cut, T* y, int n) {
+        shift(win, reach);
+        widen(row, win[0]);
+        if (cut) {
 #pragma unroll
-        for (int q = 0; q < kTile; ++q) now[q] = ahead[q];
-        if (s + kTile < steps) fetch(s + kTile);
+            for (int j = 1; j < W; ++j) empty(win[j]);
+        }
+        float pre[V];
+        convolve(win, w, bias, pre);
+        if (a.silu) {
 #pragma unroll
-        for (int q = 0; q < kTile; ++q) {
-            if (s + q >= steps) break;
-            shift(win, reach_of<W>(a));
-            widen(now[q], win[0]);
-            if (cuts >> (s + q) & 1) {
+            for (int i = 0; i < V; ++i) pre[i] *= sigmoid(pre[i]);
+        }
+        store_row(y, n, pre);
+    };
+    if (__ballot(steps < kRun || cuts || ch.n < V) == 0) {
+        const T* xw = xp + ch.c;
+        Raw<T> ahead[TT];
 #pragma unroll
-                for (int j = 1; j < W; ++j) empty(win[j]);
+        for (int q = 0; q < TT; ++q) ahead[q] = load_whole(xw + q * a.x_t);
+        load_weights<W>(a, ch, w, bias);
+        load_window<T, W>(a, b, t0, ch, win);
+#pragma unroll
+        for (int s = 0; s < kRun; s += TT) {
+            Raw<T> now[TT];
+#pragma unroll
+            for (int q = 0; q < TT; ++q) {
+                now[q] = ahead[q];
+                if (s + TT < kRun) ahead[q] = load_whole(xw + (s + TT + q) * a.x_t);
             }
-            float pre[V];
-            convolve(win, w, bias, pre);
-            if (a.silu) {
 #pragma unroll
-                for (int i = 0; i < V; ++i) pre[i] *= sigmoid(pre[i]);
-            }
-            store_row(yp + (s + q) * a.y_t, n, pre);
+            for (int q = 0; q < TT; ++q) step(now[q], false, yp + (s + q) * a.y_t, V);
+        }
+    } else {
+        load_weights<W>(a, ch, w, bias);
+        load_window<T, W>(a, b, t0, ch, win);
+        constexpr int SLOW = 4;
+        Raw<T> ahead[SLOW];
+        auto fetch = [&](int s) {
+#pragma unroll
+            for (int q = 0; q < SLOW; ++q) ahead[q] = load_raw(xp + (s + q < steps ? s + q : steps - 1) * a.x_t, ch);
+        };
+        fetch(0);
+#pragma unroll 1
+        for (int s = 0; s < steps; s += SLOW) {
+            Raw<T> now[SLOW];
+#pragma unroll
+            for (int q = 0; q < SLOW; ++q) now[q] = ahead[q];
+            fetch(s + SLOW);
+#pragma unroll
+            for (int q = 0; q < SLOW; ++q)
+                if (s + q < steps) step(now[q], cuts >> (s + q) & 1, yp + (s + q) * a.y_t, ch.n);
         }
     }
     if (a.state_out && t0 + steps == a.length) {
         // the window the next call starts from
-        T* so = (T*)a.state_out + (int64_t)b * (a.width - 1) * a.channels + c;
+        T* so = (T*)a.state_out + (int64_t)b * (a.width - 1) * a.channels + ch.c;
 #pragma unroll
         for (int j = 0; j < W - 1; ++j)
-            if (j < a.width - 1) store_row(so + (int64_t)(a.width - 2 - j) * a.channels, n, win[j]);
+            if (j < a.width - 1) store_row(so + (int64_t)(a.width - 2 - j) * a.channels, ch.n, win[j]);
     }
 }
 
@@ -268,23 +330,23 @@ constexpr int kRows = 4;
 
 template <typename T, int W>
 __global__ __launch_bounds__(kThreads) void conv_step(ConvArgs a) {
-    int c, n;
+    Chan ch;
     int64_t group;
-    if (!place(a, (a.batch + kRows - 1) / kRows, &c, &n, &group)) return;
+    if (!place(a, (a.batch + kRows - 1) / kRows, &ch, &group)) return;
     float w[W][V], bias[V];
-    load_weights<W>(a, c, n, w, bias);
     Raw<T> x[kRows], past[kRows][W];
     bool cut[kRows];
     const T* sp = (const T*)a.state;
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
         const int64_t b = group * kRows + r < a.batch ? group * kRows + r : a.batch - 1;
-        x[r] = load_raw((const T*)a.x + b * a.x_b + c, n);
+        x[r] = load_raw((const T*)a.x + b * a.x_b, ch);
         cut[r] = a.resets && a.resets[b * a.resets_b] != 0;
 #pragma unroll
         for (int j = 1; j < W; ++j)
-            if (sp && j < a.width) past[r][j] = load_raw(sp + (b * (a.width - 1) + a.width - 1 - j) * a.channels + c, n);
+            if (sp && j < a.width) past[r][j] = load_raw(sp + (b * (a.width - 1) + a.width - 1 - j) * a.channels, ch);
     }
+    load_weights<W>(a, ch, w, bias);
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
         const int64_t b = group * kRows + r;
@@ -303,12 +365,12 @@ __global__ __launch_bounds__(kThreads) void conv_step(ConvArgs a) {
 #pragma unroll
             for (int i = 0; i < V; ++i) pre[i] *= sigmoid(pre[i]);
         }
-        store_row((T*)a.y + b * a.y_b + c, n, pre);
+        store_row((T*)a.y + b * a.y_b + ch.c, ch.n, pre);
         if (a.state_out) {
-            T* so = (T*)a.state_out + b * (a.width - 1) * a.channels + c;
+            T* so = (T*)a.state_out + b * (a.width - 1) * a.channels + ch.c;
 #pragma unroll
             for (int j = 0; j < W - 1; ++j)
-                if (j < a.width - 1) store_row(so + (int64_t)(a.width - 2 - j) * a.channels, n, win[j]);
+                if (j < a.width - 1) store_row(so + (int64_t)(a.width - 2 - j) * a.channels, ch.n, win[j]);
         }
     }
 }
@@ -319,17 +381,18 @@ __global__ __launch_bounds__(kThreads) void conv_step(ConvArgs a) {
 // their gradients from.
 template <typename T, int W>
 __global__ __launch_bounds__(kThreads) void conv_backward(ConvArgs a, ConvGradArgs g) {
-    constexpr int STEPS = kRun + W - 1;
+    constexpr int STEPS = kRun + W - 1, TT = 4;
     __shared__ float lds[kThreads][V + 1];
-    int c, n;
+    Chan ch;
     int64_t share;
     const int64_t shares = (int64_t)g.rows * (kThreads / a.lanes);
-    const bool any = place(a, shares, &c, &n, &share);
+    const bool any = place(a, shares, &ch, &share);
+    const int reach = reach_of<W>(a);
     float w[W][V], bias[V], dw[W][V], db[V];
     empty(db);
 #pragma unroll
     for (int j = 0; j < W; ++j) empty(dw[j]);
-    if (any) load_weights<W>(a, c, n, w, bias);
+    if (any) load_weights<W>(a, ch, w, bias);
     for (int64_t job = any ? share : a.jobs; job < a.jobs; job += shares) {
         const int b = (int)(job / a.runs);
         const int64_t t0 = job % a.runs * kRun;
@@ -337,85 +400,125 @@ __global__ __launch_bounds__(kThreads) void conv_backward(ConvArgs a, ConvGradAr
         // steps t0 .. t0+steps-1 have a dpre; the run owns the gradients of
         // inputs t0 .. t0+own-1, the first run those of the state too
         const int steps = a.length - t0 < own + W - 1 ? (int)(a.length - t0) : own + W - 1;
-        const T* xp = (const T*)a.x + b * a.x_b + t0 * a.x_t + c;
-        const T* dyp = (const T*)g.dy + b * g.dy_b + t0 * g.dy_t + c;
-        T* dxp = (T*)g.dx + ((int64_t)b * a.length + t0) * a.channels + c;
-        Raw<T> xa[kTile], da[kTile];
-        auto fetch = [&](int s) {
-#pragma unroll
-            for (int q = 0; q < kTile; ++q) {
-                const int k = s + q < steps ? s + q : steps - 1;
-                xa[q] = load_raw(xp + k * a.x_t, n);
-                da[q] = load_raw(dyp + k * g.dy_t, n);
-            }
-        };
-        fetch(0);
-        const unsigned cuts = beginnings<STEPS>(a, b, t0);
+        const T* xp = (const T*)a.x + b * a.x_b + t0 * a.x_t;
+        const T* dyp = (const T*)g.dy + b * g.dy_b + t0 * g.dy_t;
+        T* dxp = (T*)g.dx + ((int64_t)b * a.length + t0) * a.channels + ch.c;
+        // beginnings from the window before the run on
+        const unsigned all = beginnings<STEPS + W - 1>(a, b, t0 - (W - 1));
+        const unsigned cuts = all >> (W - 1), past = all & ((1u << (W - 1)) - 1);
         float win[W][V], acc[W][V];   // acc[j]: gradient of the input j steps back, so far
-        load_window<T, W>(a, b, t0, c, n, win);
 #pragma unroll
         for (int j = 0; j < W; ++j) empty(acc[j]);
-        // how far back the step before sees; only the state's gradient and a
-        // beginning make it less than everything
-        const int reach = reach_of<W>(a);
-        int sight = reach;
-        if (t0 > 0 && a.resets) {
-            const unsigned past = beginnings<W - 1>(a, b, t0 - (W - 1));
-            const int s = past ? __clz(past << (32 - (W - 1))) : reach;
-            sight = s < reach ? s : reach;
-        }
+        // how far back the step before sees
+        int sight = past ? __clz(past << (32 - (W - 1))) : reach;
+        sight = sight < reach ? sight : reach;
         auto put = [&](int t, float (&v)[V]) {   // the gradient of input t0 + t is whole
             if (t >= 0 && t < own) {
-                store_row(dxp + (int64_t)t * a.channels, n, v);
+                store_row(dxp + (int64_t)t * a.channels, ch.n, v);
             } else if (t0 == 0 && t < 0 && g.dstate && t >= -(a.width - 1)) {
-                store_row((T*)g.dstate + ((int64_t)b * (a.width - 1) + a.width - 1 + t) * a.channels + c, n, v);
+                store_row((T*)g.dstate + ((int64_t)b * (a.width - 1) + a.width - 1 + t) * a.channels + ch.c, ch.n, v);
             }
         };
-        for (int s = 0; s < steps; s += kTile) {
-            Raw<T> xn[kTile], dn[kTile];
-#pragma unroll
-            for (int q = 0; q < kTile; ++q) xn[q] = xa[q], dn[q] = da[q];
-            if (s + kTile < steps) fetch(s + kTile);
-#pragma unroll
-            for (int q = 0; q < kTile; ++q) {
-                const int t = s + q;
-                if (t >= steps) break;
-                shift(win, reach);
-                shift(acc, W);   // the gradients go on to where they are put
-                empty(acc[0]);
-                widen(xn[q], win[0]);
+        // A step: FAST asks nothing, OWN is in the run itself.
+        auto step = [&](auto fast, auto in_run, int t, const Raw<T>& xn, const Raw<T>& dn) {
+            constexpr bool FAST = decltype(fast)::value, OWN = decltype(in_run)::value;
+            shift(win, reach);
+            shift(acc, W);   // the gradients go on to where they are put
+            empty(acc[0]);
+            widen(xn, win[0]);
+            if (!FAST) {
                 sight = sight < reach ? sight + 1 : reach;
                 if (cuts >> t & 1) {
                     sight = 0;
 #pragma unroll
                     for (int j = 1; j < W; ++j) empty(win[j]);
                 }
-                float d[V];
-                widen(dn[q], d);
-                if (a.silu) {
-                    float pre[V];
-                    convolve(win, w, bias, pre);
+            }
+            float d[V];
+            widen(dn, d);
+            if (a.silu) {
+                float pre[V];
+                convolve(win, w, bias, pre);
 #pragma unroll
-                    for (int i = 0; i < V; ++i) {
-                        const float s1 = sigmoid(pre[i]);
-                        d[i] *= s1 * __builtin_fmaf(pre[i], 1.0f - s1, 1.0f);
-                    }
+                for (int i = 0; i < V; ++i) {
+                    const float s1 = sigmoid(pre[i]);
+                    d[i] *= s1 * __builtin_fmaf(pre[i], 1.0f - s1, 1.0f);
                 }
+            }
+#pragma unroll
+            for (int j = 0; j < W; ++j)
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    const float more = __builtin_fmaf(w[j][i], d[i], acc[j][i]);
+                    acc[j][i] = FAST || j <= sight ? more : acc[j][i];
+                }
+            if (OWN && (FAST || t < own)) {
 #pragma unroll
                 for (int j = 0; j < W; ++j)
-                    if (j <= sight) {
 #pragma unroll
-                        for (int i = 0; i < V; ++i) acc[j][i] = __builtin_fmaf(w[j][i], d[i], acc[j][i]);
-                    }
-                if (t < own) {
+                    for (int i = 0; i < V; ++i) dw[j][i] = __builtin_fmaf(d[i], win[j][i], dw[j][i]);
 #pragma unroll
-                    for (int j = 0; j < W; ++j)
-#pragma unroll
-                        for (int i = 0; i < V; ++i) dw[j][i] = __builtin_fmaf(d[i], win[j][i], dw[j][i]);
-#pragma unroll
-                    for (int i = 0; i < V; ++i) db[i] += d[i];
-                }
+                for (int i = 0; i < V; ++i) db[i] += d[i];
+            }
+            if (!FAST || (OWN && t < W - 1))
                 put(t - (W - 1), acc[W - 1]);
+            else
+                store_row(dxp + (int64_t)(t - (W - 1)) * a.channels, V, acc[W - 1]);
+        };
+        // (widths that the template only covers keep to the copy that asks)
+        if (W < kMaxWidth && __ballot(steps < STEPS || cuts || past || ch.n < V) == 0) {
+            Raw<T> xa[TT], da[TT];
+            const T *xw = xp + ch.c, *dw_ = dyp + ch.c;
+            auto fetch = [&](int count) {   // the next rows
+#pragma unroll
+                for (int q = 0; q < TT; ++q) {
+                    if (q >= count) break;
+                    xa[q] = load_whole(xw);
+                    da[q] = load_whole(dw_);
+                    xw += a.x_t;
+                    dw_ += g.dy_t;
+                }
+            };
+            fetch(TT);
+            load_window<T, W>(a, b, t0, ch, win);
+#pragma unroll 1
+            for (int s = 0; s < kRun; s += TT) {
+                Raw<T> xn[TT], dn[TT];
+#pragma unroll
+                for (int q = 0; q < TT; ++q) xn[q] = xa[q], dn[q] = da[q];
+                if (s + TT < kRun)
+                    fetch(TT);
+                else
+                    fetch(W - 1);
+#pragma unroll
+                for (int q = 0; q < TT; ++q) step(std::true_type(), std::true_type(), s + q, xn[q], dn[q]);
+            }
+#pragma unroll
+            for (int q = 0; q < W - 1 && q < TT; ++q) step(std::true_type(), std::false_type(), kRun + q, xa[q], da[q]);
+        } else {
+            load_window<T, W>(a, b, t0, ch, win);
+            Raw<T> xa[TT], da[TT];
+            auto fetch = [&](int s) {
+#pragma unroll
+                for (int q = 0; q < TT; ++q) {
+                    const int k = s + q < steps ? s + q : steps - 1;
+                    xa[q] = load_raw(xp + k * a.x_t, ch);
+                    da[q] = load_raw(dyp + k * g.dy_t, ch);
+                }
+            };
+            fetch(0);
+#pragma unroll 1
+            for (int s = 0; s < steps; s += TT) {
+                Raw<T> xn[TT], dn[TT];
+#pragma unroll
+                for (int q = 0; q < TT; ++q) xn[q] = xa[q], dn[q] = da[q];
+                fetch(s + TT);
+#pragma unroll 1
+                for (int q = 0; q < TT && s + q < steps; ++q) {
+                    step(std::false_type(), std::true_type(), s + q, xn[0], dn[0]);
+#pragma unroll
+                    for (int k = 0; k + 1 < TT; ++k) xn[k] = xn[k + 1], dn[k] = dn[k + 1];
+                }
             }
         }
         if (t0 + steps == a.length) {
@@ -425,8 +528,8 @@ __global__ __launch_bounds__(kThreads) void conv_backward(ConvArgs a, ConvGradAr
             for (int j = W - 2; j >= 0; --j) {
                 if (g.dstate_out && j < a.width - 1 && j <= sight) {
                     float v[V];
-                    widen(load_raw((const T*)g.dstate_out +
-                                       ((int64_t)b * (a.width - 1) + a.width - 2 - j) * a.channels + c, n), v);
+                    widen(load_raw((const T*)g.dstate_out + ((int64_t)b * (a.width - 1) + a.width - 2 - j) * a.channels,
+                                   ch), v);
 #pragma unroll
                     for (int i = 0; i < V; ++i) acc[j][i] += v[i];
                 }
@@ -453,7 +556,7 @@ __global__ __launch_bounds__(kThreads) void conv_backward(ConvArgs a, ConvGradAr
                 for (int i = 0; i < V; ++i) s[i] += lds[threadIdx.x + k * a.lanes][i];
 #pragma unroll
             for (int i = 0; i < V; ++i)
-                if (any && i < n) out[(int64_t)(j < W ? j : a.width) * a.channels + c + i] = s[i];
+                if (any && i < ch.n) out[(int64_t)(j < W ? j : a.width) * a.channels + ch.c + i] = s[i];
         }
     }
 }
