@@ -132,6 +132,11 @@ def _rows(t):
     return t.data_ptr(), s[0], s[1]
 
 
+def _like(t):
+    """A new dense tensor of t's shape and type; of none, none."""
+    return None if t is None else torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
 def _row(t):
     """The same of a (batch, ...) tensor: one step."""
     return (0, 0, 0) if t is None else (t.data_ptr(), t.stride(0), 0)
@@ -156,8 +161,8 @@ def _wants_grad(*tensors) -> bool:
 
 def _conv(x, weight, bias, state, resets, silu):
     b, n, d = x.shape
-    y = torch.empty((b, n, d), dtype=x.dtype, device=x.device)
-    state_out = torch.empty((b, weight.shape[1] - 1, d), dtype=x.dtype, device=x.device)
+    y = _like(x)
+    state_out = x.new_empty((b, weight.shape[1] - 1, d))
     _call(x.get_device(), "sdfr_conv", _conv_desc(x, weight, bias, silu, resets, state, y, state_out))
     return y, state_out
 
@@ -179,10 +184,7 @@ class _CausalConv(torch.autograd.Function):
         dy = torch.zeros_like(x) if dy is None else dy if dy.stride(-1) == 1 or d == 1 else dy.contiguous()
         if dstate_out is not None:
             dstate_out = dstate_out.contiguous()
-        dx = torch.empty((b, n, d), dtype=x.dtype, device=x.device)
-        dweight = torch.empty_like(weight)
-        dbias = torch.empty_like(bias) if bias is not None else None
-        dstate = torch.empty_like(state) if state is not None else None
+        dx, dweight, dbias, dstate = _like(x), _like(weight), _like(bias), _like(state)
         desc = _conv_desc(x, weight, bias, ctx.silu, resets, state, dx, None)
         ws = _workspace(_sdfr.packed("sdfr_conv_grad_workspace_bytes")(desc), x.device)
         grad = _sdfr.ConvGrad.pack(*_rows(dy), _ptr(dstate_out), dx.data_ptr(), _ptr(dstate), dweight.data_ptr(),
@@ -230,7 +232,7 @@ def causal_conv_step(x, state, weight, bias=None, *, silu: bool = True, resets=N
     state = _target("state", state, past, x.dtype, x, True)
     state_out = state if state_out is None else _target("state_out", state_out, past, x.dtype, x, True)
     resets = _resets(resets, (b,), x)
-    y = torch.empty((b, d), dtype=x.dtype, device=x.device) if out is None \
+    y = _like(x) if out is None \
         else _target("out", out, (b, d), x.dtype, x, False)
     if b and d:
         _call(x.get_device(), "sdfr_conv",
@@ -240,23 +242,28 @@ def causal_conv_step(x, state, weight, bias=None, *, silu: bool = True, resets=N
 
 
 # --------------------------------------------------------------------- scan --
-def _scan_desc(x, dt, A, B, C, D, z, dt_bias, softplus, resets, state, y, state_out, marks):
+def _scan_fields(x, dt, A, B, C, D, z, dt_bias, softplus, resets, state, y, state_out, marks):
     b, n, d = x.shape
-    return _sdfr.Scan.pack(*_rows(x), *_rows(dt), *_rows(z), *_rows(B), *_rows(C), A.data_ptr(), _ptr(D),
-                           _ptr(dt_bias), *_rows(resets), _ptr(state), _ptr(state_out), _ptr(marks), *_rows(y), n, b,
-                           d, A.shape[1], _CODES[x.dtype], 1 if softplus else 0)
+    return [*_rows(x), *_rows(dt), *_rows(z), *_rows(B), *_rows(C), A.data_ptr(), _ptr(D), _ptr(dt_bias),
+            *_rows(resets), _ptr(state), _ptr(state_out), _ptr(marks), *_rows(y), n, b, d, A.shape[1],
+            _CODES[x.dtype], 1 if softplus else 0]
+
+
+_MARKS = [w.split(":")[0] for w in _sdfr._SCAN.split()].index("marks")
 
 
 def _scan(x, dt, A, B, C, D, z, dt_bias, state, resets, softplus, keep=False):
     """y, the final state, and with ``keep`` what the gradients start from."""
     b, n, d = x.shape
-    y = torch.empty((b, n, d), dtype=x.dtype, device=x.device)
-    state_out = torch.empty((b, d, A.shape[1]), dtype=torch.float32, device=x.device)
+    y = _like(x)
+    state_out = x.new_empty((b, d, A.shape[1]), dtype=torch.float32)
     marks = None
-    desc = _scan_desc(x, dt, A, B, C, D, z, dt_bias, softplus, resets, state, y, state_out, None)
+    fields = _scan_fields(x, dt, A, B, C, D, z, dt_bias, softplus, resets, state, y, state_out, None)
+    desc = _sdfr.Scan.pack(*fields)
     if keep:
         marks = _workspace(_sdfr.packed("sdfr_scan_marks_bytes")(desc), x.device)
-        desc = _scan_desc(x, dt, A, B, C, D, z, dt_bias, softplus, resets, state, y, state_out, marks)
+        fields[_MARKS] = marks.data_ptr()
+        desc = _sdfr.Scan.pack(*fields)
     ws = _workspace(_sdfr.packed("sdfr_scan_workspace_bytes")(desc, 0), x.device)
     _call(x.get_device(), "sdfr_scan", desc, ws.data_ptr(), ws.numel())
     return (y, state_out, marks) if keep else (y, state_out)
@@ -280,12 +287,10 @@ class _SelectiveScan(torch.autograd.Function):
         if dstate_out is not None:
             dstate_out = dstate_out.contiguous()
 
-        def like(t):
-            return torch.empty(t.shape, dtype=t.dtype, device=t.device) if t is not None else None
-
-        dx, ddt, dz, dB, dC = like(x), like(dt), like(z), like(B), like(C)
-        dA, dD, dbias, dstate = like(A), like(D), like(dt_bias), like(state)
-        desc = _scan_desc(x, dt, A, B, C, D, z, dt_bias, ctx.softplus, resets, state, dx, None, marks)
+        dx, ddt, dz, dB, dC = _like(x), _like(dt), _like(z), _like(B), _like(C)
+        dA, dD, dbias, dstate = _like(A), _like(D), _like(dt_bias), _like(state)
+        desc = _sdfr.Scan.pack(*_scan_fields(x, dt, A, B, C, D, z, dt_bias, ctx.softplus, resets, state, dx, None,
+                                             marks))
         ws = _workspace(_sdfr.packed("sdfr_scan_workspace_bytes")(desc, 1), x.device)
         grad = _sdfr.ScanGrad.pack(*_rows(dout), _ptr(dstate_out), dx.data_ptr(), ddt.data_ptr(), _ptr(dz),
                               dB.data_ptr(), dC.data_ptr(), dA.data_ptr(), _ptr(dD), _ptr(dbias), _ptr(dstate))
@@ -350,7 +355,7 @@ def selective_scan_step(x, dt, A, B, C, state, *, D=None, z=None, dt_bias=None, 
     state = _target("state", state, (b, d, m), torch.float32, x, True)
     state_out = state if state_out is None else _target("state_out", state_out, (b, d, m), torch.float32, x, True)
     resets = _resets(resets, (b,), x)
-    y = torch.empty((b, d), dtype=x.dtype, device=x.device) if out is None \
+    y = _like(x) if out is None \
         else _target("out", out, (b, d), x.dtype, x, False)
     if b and d:
         _call(x.get_device(), "sdfr_scan",
