@@ -352,22 +352,29 @@ __global__ __launch_bounds__(256) void draw_small(DrawArgs a) {
 // one in which the count or the mass passes its bound, and within that bin the
 // keys are ranked against each other (or, where there are too many of them,
 // fall into bins by key until one bin holds a single key or few enough).
-// Bins first take the nearest kNear only, where the answer nearly always lies,
-// so most candidates cost no LDS operation; beyond kFar weights are zero, and
-// a threshold there is none. Sums are of integers, so the order in which the
-// LDS takes them does not matter.
+// Beyond kFar weights are zero, and a threshold there is none. Sums are of
+// integers, so the order in which the LDS takes them does not matter.
+//
+// Most draws need a fraction of a row, and all that follows happens on a list
+// of it, if it fits the LDS: with top-k the candidates down to where at least k
+// of them lie, going by the largest of each of a few thousand groups, which the
+// pass that finds the largest of all keeps; with top-p alone those down to the
+// bin of the threshold; with min-p alone those above that.
 //
 // A top-p threshold after a top-k one needs no list of what top-k left: its
 // bound is a share of that mass, which is reached at or above the top-k key,
 // and among the ties there no later than the last one taken.
-constexpr int kBins = 2048, kList = 256;
+constexpr int kList = 256, kGroups = 4;   // keys ranked against each other; maxima a thread keeps
 constexpr float kNear = 8.0f, kFar = 28.0f;
+enum { kRangeNear, kRangeFar, kRangeAll };   // what the bins spread over: up to kNear, from there to kFar, up to kFar
 
 template <int THREADS>
 struct Shared {
+    static constexpr int kBins = THREADS * 4, kCandidates = THREADS * 4;
     u64 mass[kBins];
     uint32_t count[kBins];
     uint32_t list[kList];
+    uint32_t key_of[kCandidates], index_of[kCandidates];
     u64 part[THREADS / 64], part2[THREADS / 64];
     u64 turn[THREADS];            // kept mass of each turn of each wave
     int ties[THREADS];            // and its candidates at the threshold
@@ -381,7 +388,8 @@ __device__ __forceinline__ void one_by_one() { __builtin_amdgcn_sched_barrier(0)
 
 template <typename T, int THREADS>
 struct Block {
-    static constexpr int V = Row<T>::V, WAVES = THREADS / 64, N = kBins / THREADS;
+    static constexpr int kBins = Shared<THREADS>::kBins, kCandidates = Shared<THREADS>::kCandidates;
+    static constexpr int V = Row<T>::V, WAVES = THREADS / 64, N = kBins / THREADS, kAhead = 4;
     const Row<T> r;
     Shared<THREADS>& sh;
     const Settings& s;
@@ -389,14 +397,14 @@ struct Block {
     int turns;              // of each wave
     float m, inv_t;
     int have = -1;          // the range whose bins are in LDS
-    u64 low = 0;            // this thread's mass beyond kNear
+    int listed = 0;         // candidates in the list, if the rest happens there
 
     __device__ __forceinline__ Block(const DrawArgs& a, int row, Shared<THREADS>& shared, const Settings& settings)
         : r(a, row), sh(shared), s(settings), lane(threadIdx.x & 63), wave(threadIdx.x / 64) {
         const int all = (a.vocab + 64 * V - 1) / (64 * V);
         turns = (all + WAVES - 1) / WAVES;
     }
-    // Calls f(turn, logits) for the wave's turns in order, with all lanes; the next three turns' loads are in flight.
+    // Calls f(turn, logits) for the wave's turns in order, with all lanes; the next few turns' loads are in flight.
     template <class F>
     __device__ __forceinline__ void each(F f) const {
         // where the lane starts is worked out anew by every pass: kept, it and what follows from it would be held in
@@ -404,16 +412,33 @@ struct Block {
         int start = (wave * turns * 64 + lane) * V;
         asm volatile("" : "+v"(start));
         auto index = [&](int turn) { return start + turn * 64 * V; };
-        typename Row<T>::Vec ahead[3] = {r.load(index(0)), r.load(index(1)), r.load(index(2))};
+        typename Row<T>::Vec ahead[kAhead];
+#pragma unroll
+        for (int q = 0; q < kAhead; ++q) ahead[q] = r.load(index(q));
 #pragma unroll 1
         for (int t = 0; t < turns; ++t) {
             float x[V];
 #pragma unroll
             for (int j = 0; j < V; ++j) x[j] = ahead[0][j];
-            ahead[0] = ahead[1];
-            ahead[1] = ahead[2];
-            ahead[2] = r.load(index(t + 3));
+#pragma unroll
+            for (int q = 0; q + 1 < kAhead; ++q) ahead[q] = ahead[q + 1];
+            ahead[kAhead - 1] = r.load(index(t + kAhead));
             f(t, x);
+        }
+    }
+    // Calls f(logit) for every candidate, of the list if there is one, in any order.
+    template <class F>
+    __device__ __forceinline__ void candidates(F f) const {
+        if (listed) {
+            for (int i = threadIdx.x; i < listed; i += THREADS) f(of_key(sh.key_of[i]));
+        } else {
+            each([&](int, float(&x)[V]) {
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    one_by_one();
+                    f(x[j]);
+                }
+            });
         }
     }
     __device__ __forceinline__ float z(float x) const { return z_of(x, m, inv_t); }
@@ -446,47 +471,47 @@ struct Block {
         return before;
     }
 
+    // Empty bins, and an empty list.
     __device__ __forceinline__ void clear() {
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < N; ++i) sh.mass[threadIdx.x + i * THREADS] = 0, sh.count[threadIdx.x + i * THREADS] = 0;
+        for (int i = 0; i < N; ++i) {
+            sh.count[threadIdx.x + i * THREADS] = 0;
+            if (s.cut) sh.mass[threadIdx.x + i * THREADS] = 0;
+        }
+        if (threadIdx.x == 0) sh.fill = 0, sh.lo = 0xffffffffu, sh.hi = 0;
+        __syncthreads();
+    }
+    __device__ __forceinline__ void clear_list() {
+        __syncthreads();
         if (threadIdx.x == 0) sh.fill = 0, sh.lo = 0xffffffffu, sh.hi = 0;
         __syncthreads();
     }
     // Distances (from, to] of a range, and its bins; -1: outside.
     __device__ __forceinline__ static int bin_of(float z, int range) {
-        const float from = range ? kNear : 0.0f, to = range ? kFar : kNear;
-        if (!(z > -to) || (range && z > -from)) return -1;
+        const float from = range == kRangeFar ? kNear : 0.0f, to = range == kRangeNear ? kNear : kFar;
+        if (!(z > -to) || (range == kRangeFar && z > -from)) return -1;
         const int b = (int)((-z - from) * (kBins / (to - from)));
         return b < kBins ? b : kBins - 1;
     }
-    // Fills the bins with a range. With top-p, masses too, and the first time
-    // the mass of what lies further off.
-    __device__ __forceinline__ void fill(int range, bool want_low) {
+    // Fills the bins with a range; with top-p, masses too.
+    __device__ __forceinline__ void fill(int range) {
         clear();
-        u64 l = 0;
-        each([&](int, float(&x)[V]) {
-#pragma unroll
-            for (int j = 0; j < V; ++j) {
-                one_by_one();
-                const float zj = z(x[j]);
-                const int b = bin_of(zj, range);
-                if (b >= 0) {
-                    atomicAdd(&sh.count[b], 1u);
-                    if (s.cut) atomicAdd(&sh.mass[b], weight(expf(zj)));
-                } else if (want_low && zj > -kFar) {
-                    l += weight(expf(zj));
-                }
+        candidates([&](float x) {
+            const float zx = z(x);
+            const int b = bin_of(zx, range);
+            if (b >= 0) {
+                atomicAdd(&sh.count[b], 1u);
+                if (s.cut) atomicAdd(&sh.mass[b], weight(expf(zx)));
             }
         });
-        if (want_low) low = l;
         have = range;
         __syncthreads();
     }
     __device__ __forceinline__ void totals(u64* c, u64* v) const {
         u64 tc = 0, tv = 0;
 #pragma unroll
-        for (int i = 0; i < N; ++i) tc += sh.count[threadIdx.x + i * THREADS], tv += sh.mass[threadIdx.x + i * THREADS];
+        for (int i = 0; i < N; ++i) tc += sh.count[threadIdx.x + i * THREADS], tv += s.cut ? sh.mass[threadIdx.x + i * THREADS] : 0;
         *c = sum(tc);
         *v = sum(tv);
     }
@@ -499,7 +524,7 @@ struct Block {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             c[i] = sh.count[threadIdx.x * N + i];
-            v[i] = sh.mass[threadIdx.x * N + i];
+            v[i] = s.cut ? sh.mass[threadIdx.x * N + i] : 0;
             cs += c[i];
             vs += v[i];
         }
@@ -522,19 +547,15 @@ struct Block {
     // Keys of one bin, between lo and hi, into the list if they fit, and their
     // lowest and highest.
     __device__ __forceinline__ void collect(int range, int bin, uint32_t lo, uint32_t hi, uint32_t members) {
-        clear();
+        clear_list();
         have = -1;
-        each([&](int, float(&x)[V]) {
-#pragma unroll
-            for (int j = 0; j < V; ++j) {
-                one_by_one();
-                if (bin_of(z(x[j]), range) == bin) {
-                    const uint32_t k = key_of(x[j]);
-                    if (k >= lo && k <= hi) {
-                        if (members <= kList) sh.list[atomicAdd(&sh.fill, 1u)] = k;
-                        atomicMin(&sh.lo, k);
-                        atomicMax(&sh.hi, k);
-                    }
+        candidates([&](float x) {
+            if (bin_of(z(x), range) == bin) {
+                const uint32_t k = key_of(x);
+                if (k >= lo && k <= hi) {
+                    if (members <= kList) sh.list[atomicAdd(&sh.fill, 1u)] = k;
+                    atomicMin(&sh.lo, k);
+                    atomicMax(&sh.hi, k);
                 }
             }
         });
@@ -545,12 +566,12 @@ struct Block {
     // among weights of zero.
     __device__ __forceinline__ bool threshold(bool by_mass, u64 bound, Cut* cut, u64* kept) {
         u64 above_c = 0, above_m = 0;
-        int range = 0;
-        if (have != 0) fill(0, false);
+        int range = have;
+        if (range < 0) fill(range = by_mass ? kRangeAll : kRangeNear);
         if (!find(by_mass, bound)) {
+            if (range != kRangeNear) return false;
             totals(&above_c, &above_m);
-            fill(1, false);
-            range = 1;
+            fill(range = kRangeFar);
             if (!find(by_mass, bound - (by_mass ? above_m : above_c))) return false;
         }
         const int bin = (int)sh.bin;
@@ -563,16 +584,12 @@ struct Block {
             int shift = 0;
             while ((hi - lo) >> shift >= (uint32_t)kBins) ++shift;
             clear();
-            each([&](int, float(&x)[V]) {
-#pragma unroll
-                for (int j = 0; j < V; ++j) {
-                    one_by_one();
-                    if (bin_of(z(x[j]), range) == bin) {
-                        const uint32_t k = key_of(x[j]);
-                        if (k >= lo && k <= hi) {
-                            atomicAdd(&sh.count[(hi - k) >> shift], 1u);
-                            if (s.cut) atomicAdd(&sh.mass[(hi - k) >> shift], w(x[j]));
-                        }
+            candidates([&](float x) {
+                if (bin_of(z(x), range) == bin) {
+                    const uint32_t k = key_of(x);
+                    if (k >= lo && k <= hi) {
+                        atomicAdd(&sh.count[(hi - k) >> shift], 1u);
+                        if (s.cut) atomicAdd(&sh.mass[(hi - k) >> shift], w(x));
                     }
                 }
             });
@@ -619,6 +636,54 @@ struct Block {
         *kept = sh.mass_kept;
         return true;
     }
+    // A logit that at least `want` candidates reach, going by the threads' group
+    // maxima; false if none is found within kNear.
+    __device__ __forceinline__ bool bound_of(const float (&group)[kGroups], int want, float* bound) {
+        clear();
+        have = -1;
+#pragma unroll
+        for (int q = 0; q < kGroups; ++q) {
+            const int b = bin_of(z(group[q]), kRangeNear);
+            if (b >= 0) atomicAdd(&sh.count[b], 1u);
+        }
+        if (!find(false, (u64)want)) return false;
+        *bound = logit_below(sh.bin, kNear);
+        return true;
+    }
+    // A logit no higher than those of a bin of a range from 0 `to`. (A list may
+    // hold more than it has to, so what is rounded off goes to be safe.)
+    __device__ __forceinline__ float logit_below(uint32_t bin, float to) const {
+        return m - (float)(bin + 2) * (to / kBins) / inv_t;
+    }
+    // Lists the candidates that reach `bound`; false (and nothing listed) where
+    // they do not fit or are fewer than `want`.
+    __device__ __forceinline__ bool make_list(float bound, int want) {
+        clear_list();
+        have = -1;
+        each([&](int t, float(&x)[V]) {
+            int mine = 0;
+#pragma unroll
+            for (int j = 0; j < V; ++j) mine += x[j] >= bound;
+            if (__ballot(mine != 0)) {
+                const int upto = (int)wave_scan((u64)mine);
+                int at = 0;
+                if (lane == 63) at = (int)atomicAdd(&sh.fill, (uint32_t)upto);
+                at = __builtin_amdgcn_readlane(at, 63) + upto - mine;
+                const int i = ((wave * turns + t) * 64 + lane) * V;
+#pragma unroll
+                for (int j = 0; j < V; ++j)
+                    if (x[j] >= bound) {
+                        if (at < kCandidates) sh.key_of[at] = key_of(x[j]), sh.index_of[at] = (uint32_t)(i + j);
+                        ++at;
+                    }
+            }
+        });
+        __syncthreads();
+        const int n = (int)sh.fill;
+        if (n > kCandidates || n < want) return false;
+        listed = n;
+        return true;
+    }
 };
 
 template <typename T, int THREADS>
@@ -631,15 +696,30 @@ __global__ __launch_bounds__(THREADS) void draw_large(DrawArgs a) {
     B b(a, row, sh, s);
 
     // the largest, and whether anything is not a number
-    float m = -INFINITY;
+    float m = -INFINITY, group[kGroups];
+    int first = 0;   // the turn in which this thread first met its largest
     bool bad = false;
-    b.each([&](int, float(&x)[V]) {
+#pragma unroll
+    for (int q = 0; q < kGroups; ++q) group[q] = -INFINITY;
+    b.each([&](int t, float(&x)[V]) {
+        float top = x[0];
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            m = fmaxf(m, x[j]);
+            top = fmaxf(top, x[j]);
             bad |= x[j] != x[j];
         }
+        if (top > m) {
+            m = top;
+            first = t;
+        }
+        group[0] = fmaxf(group[0], top);
+        if ((t + 1) * kGroups / b.turns != t * kGroups / b.turns && t + 1 < b.turns) {   // on to the next group
+#pragma unroll
+            for (int q = kGroups - 1; q > 0; --q) group[q] = group[q - 1];
+            group[0] = -INFINITY;
+        }
     });
+    const float mine_top = m;
 #pragma unroll
     for (int d = 32; d > 0; d /= 2) m = fmaxf(m, __shfl_xor(m, d));
     const bool any_bad = __ballot(bad) != 0;
@@ -657,33 +737,115 @@ __global__ __launch_bounds__(THREADS) void draw_large(DrawArgs a) {
     b.m = m;
     b.inv_t = s.greedy ? 1.0f : s.inv_t;
 
+    if (s.greedy || s.k == 1) {   // the first of the largest
+        if (threadIdx.x == 0) sh.lo = 0xffffffffu;
+        __syncthreads();
+        const uint32_t at = (uint32_t)((b.wave * b.turns + first) * 64 + b.lane);
+        if (mine_top == m) atomicMin(&sh.lo, at);
+        __syncthreads();
+        if (mine_top == m && sh.lo == at) {
+            const auto x = b.r.load((int)at * V);
+            int j = V - 1;
+#pragma unroll
+            for (int q = V - 1; q >= 0; --q) j = x[q] == m ? q : j;
+            answer(a, row, (int64_t)at * V + j, 0.0f);
+        }
+        return;
+    }
     Cut cut = {0, ~0ull};
-    if (s.greedy || s.k == 1) {
-        cut = {key_of(m), 1};
-    } else {
+    {
         u64 kept = 0;
         bool of_k = false;
-#pragma unroll 1
-        for (int by_mass = s.k > 0 ? 0 : 1; by_mass < (s.cut ? 2 : 1); ++by_mass) {
-            u64 bound = (u64)s.k;
-            if (by_mass) {
-                if (!of_k) {   // a share of all there is
-                    b.fill(0, true);
-                    u64 c, v;
-                    b.totals(&c, &v);
-                    kept = v + b.sum(b.low);
-                }
-                bound = share(s.p24, kept, true);
-                if (bound == 0) bound = 1;
+        float bound;
+        constexpr int kMost = THREADS * kGroups / 2;   // half the groups: their maxima still tell
+        if (s.k > 0) {
+            if (s.k <= kMost && b.bound_of(group, s.k, &bound)) b.make_list(bound, s.k);
+            of_k = b.threshold(false, (u64)s.k, &cut, &kept);
+        }
+        if (s.cut) {
+            b.have = -1;
+            if (!of_k) {   // a share of all there is
+                b.listed = 0;
+                b.fill(kRangeAll);
+                u64 count;
+                b.totals(&count, &kept);
             }
-            of_k = b.threshold(by_mass != 0, bound, &cut, &kept);
+            u64 share_of = share(s.p24, kept, true);
+            if (share_of == 0) share_of = 1;
+            if (!of_k && b.find(true, share_of) && sh.above_count + sh.count[sh.bin] <= B::kCandidates &&
+                b.make_list(b.logit_below(sh.bin, kFar), 1)) {
+                // (rounding at logits of a million and more could leave some out)
+                u64 mass = 0;
+                b.candidates([&](float x) { mass += b.w(x); });
+                if (b.sum(mass) < share_of) b.listed = 0;
+            }
+            b.threshold(true, share_of, &cut, &kept);
+        } else if (!of_k && s.min_p > 0.0f) {
+            b.listed = 0;
+            // and a little more, if that is more than what is rounded off
+            if (fabsf(m) * b.inv_t < 2e4f) b.make_list(m + (logf(s.min_p) - 0.01f) / b.inv_t, 1);
         }
     }
 
-    // each turn's kept mass, and its candidates at the threshold
+    const float tie_e = expf(b.z(of_key(cut.key)));
+    const u64 tie = tie_e >= s.min_p ? weight(tie_e) : 0;
     sh.turn[threadIdx.x] = 0;
     sh.ties[threadIdx.x] = 0;
     __syncthreads();
+    if (b.listed) {
+        // all that is kept is in the list, unless only some of the ties are (the
+        // first ones, which the row knows): the kept mass of each stretch of
+        // indices, the stretch that holds the answer, and in it the candidates
+        int width = 0;   // bits of a stretch
+        while ((a.vocab - 1) >> width >= THREADS) ++width;
+        u64 ties = 0;
+        for (int i = threadIdx.x; i < b.listed; i += THREADS) {
+            const uint32_t k = sh.key_of[i];
+            ties += k == cut.key;
+            if (k >= cut.key) {
+                const float e = expf(b.z(of_key(k)));
+                if (e >= s.min_p) atomicAdd(&sh.turn[sh.index_of[i] >> width], weight(e));
+            }
+        }
+        if (b.sum(ties) <= cut.take) {   // (its barriers end the sums above)
+            const u64 mine = sh.turn[threadIdx.x];
+            u64 total;
+            const u64 before = b.scan(mine, &total);
+            const u64 target = share(chance_of(a.uniform[row]), total, false);
+            if (before <= target && target < before + mine) {   // one thread
+                sh.at = threadIdx.x;
+                sh.before = before;
+                sh.fill = 0;
+            }
+            __syncthreads();
+            const uint32_t at = sh.at;
+            u64* kept_w = sh.mass;   // of the stretch's candidates, at most 256
+            for (int i = threadIdx.x; i < b.listed; i += THREADS) {
+                const uint32_t k = sh.key_of[i], x = sh.index_of[i];
+                if (x >> width != at || k < cut.key) continue;
+                const float e = expf(b.z(of_key(k)));
+                if (!(e >= s.min_p)) continue;
+                const uint32_t q = atomicAdd(&sh.fill, 1u);
+                sh.list[q] = x;
+                sh.count[q] = k;
+                kept_w[q] = weight(e);
+            }
+            __syncthreads();
+            const int n = (int)sh.fill;
+            if ((int)threadIdx.x >= n) return;
+            const uint32_t x = sh.list[threadIdx.x];
+            u64 run = sh.before;
+            for (int i = 0; i < n; ++i)
+                if (sh.list[i] < x) run += kept_w[i];
+            if (run <= target && target < run + kept_w[threadIdx.x])
+                answer(a, row, x, s.greedy ? 0.0f : logp_of(b.z(of_key(sh.count[threadIdx.x])), total));
+            return;
+        }
+        sh.turn[threadIdx.x] = 0;
+        __syncthreads();
+    }
+
+    // each turn's kept mass, and its candidates at the threshold
     b.each([&](int t, float(&x)[V]) {
         u64 sum = 0;
         int eq = 0;
@@ -703,8 +865,6 @@ __global__ __launch_bounds__(THREADS) void draw_large(DrawArgs a) {
             sh.ties[b.wave * b.turns + t] = eq;
         }
     });
-    const float tie_e = expf(b.z(of_key(cut.key)));
-    const u64 tie = tie_e >= s.min_p ? weight(tie_e) : 0;
     __syncthreads();
     const u64 eq = sh.ties[threadIdx.x];
     u64 total;
