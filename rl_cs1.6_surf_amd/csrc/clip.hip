@@ -34,11 +34,11 @@ struct Span {
     int n, dtype;
 };
 
-__device__ inline Span span_of(const ClipTable& t) {
+__device__ inline Span span_of(const ClipTable& t, uint32_t block) {
     int lo = 0, hi = t.count;      // the last tensor whose first block is not past this one
     while (hi - lo > 1) {
         const int mid = (lo + hi) / 2;
-        if (t.first[mid] <= blockIdx.x)
+        if (t.first[mid] <= block)
             lo = mid;
         else
             hi = mid;
@@ -47,7 +47,7 @@ __device__ inline Span span_of(const ClipTable& t) {
     s.in = t.in[lo];
     s.out = t.out[lo];
     s.dtype = t.dtype[lo];
-    s.from = (int64_t)(blockIdx.x - t.first[lo]) * t.chunk;
+    s.from = (int64_t)(block - t.first[lo]) * t.chunk;
     const int64_t left = t.size[lo] - s.from;
     s.n = left < t.chunk ? (int)left : t.chunk;
     return s;
@@ -87,7 +87,7 @@ __device__ inline double block_sum(double v, double* lds) {
 
 __global__ __launch_bounds__(kThreads) void clip_squares(ClipTable t, double* parts) {
     __shared__ double lds[kThreads / 64];
-    const Span s = span_of(t);
+    const Span s = span_of(t, blockIdx.x);
     const double v = s.dtype == SDFR_F32 ? squares<float>(s) : s.dtype == SDFR_F16 ? squares<_Float16>(s)
                                                                                   : squares<__bf16>(s);
     const double sum = block_sum(v, lds);
@@ -123,7 +123,7 @@ __device__ inline void scale(const Span& s, float f) {
 }
 
 __global__ __launch_bounds__(kThreads) void clip_scale(ClipTable t, const float* factor) {
-    const Span s = span_of(t);
+    const Span s = span_of(t, gridDim.x - 1 - blockIdx.x);
     const float f = *factor;
     if (f == 1.0f && s.in == s.out) return;   // in place and within the norm: nothing changes
     if (s.dtype == SDFR_F32)
@@ -188,32 +188,39 @@ SDFR_API int32_t sdfr_clip(const SdfrTensor* tensors, int32_t count, double max_
     hipStream_t st = (hipStream_t)stream;
     float* factor = (float*)workspace;
     double* parts = (double*)((uint8_t*)workspace + 64);
-    for (int pass = 0; pass < 2; ++pass) {
-        int64_t done = 0;
-        for (int32_t i = 0; i < count;) {
-            ClipTable t;
-            t.chunk = chunk;
-            t.count = 0;
-            uint32_t at = 0;
-            for (; i < count && t.count < kTensors; ++i) {
-                if (tensors[i].size == 0) continue;
-                const int k = t.count++;
-                t.in[k] = tensors[i].in;
-                t.out[k] = tensors[i].out;
-                t.size[k] = tensors[i].size;
-                t.dtype[k] = (uint8_t)tensors[i].dtype;
-                t.first[k] = at;
-                at += (uint32_t)((tensors[i].size + chunk - 1) / chunk);
-            }
-            if (t.count == 0) break;
-            t.first[t.count] = at;
-            if (pass == 0)
-                clip_squares<<<at, kThreads, 0, st>>>(t, parts + done);
-            else
-                clip_scale<<<at, kThreads, 0, st>>>(t, factor);
-            done += at;
+    // fills a table with tensors i to end - 1; returns its blocks
+    ClipTable t;
+    t.chunk = chunk;
+    auto fill = [&](int32_t i, int32_t end) {
+        t.count = 0;
+        uint32_t at = 0;
+        for (; i < end; ++i) {
+            if (tensors[i].size == 0) continue;
+            const int k = t.count++;
+            t.in[k] = tensors[i].in;
+            t.out[k] = tensors[i].out;
+            t.size[k] = tensors[i].size;
+            t.dtype[k] = (uint8_t)tensors[i].dtype;
+            t.first[k] = at;
+            at += (uint32_t)((tensors[i].size + chunk - 1) / chunk);
         }
-        if (pass == 0) clip_norm<<<1, 1024, 0, st>>>(parts, blocks, max_norm, eps, norm, factor);
+        t.first[t.count] = at;
+        return at;
+    };
+    int64_t done = 0;
+    for (int32_t i = 0; i < count; i += kTensors) {
+        const uint32_t n = fill(i, count - i < kTensors ? count : i + kTensors);
+        if (n) clip_squares<<<n, kThreads, 0, st>>>(t, parts + done);
+        done += n;
+    }
+    clip_norm<<<1, 1024, 0, st>>>(parts, blocks, max_norm, eps, norm, factor);
+    // from the end, so that what the squares have left in the Infinity Cache is
+    // still there: whole tables of tensors, the first one with what is left over
+    for (int32_t end = count; end > 0;) {
+        const int32_t start = end > kTensors ? end - kTensors : 0;
+        const uint32_t n = fill(start, end);
+        if (n) clip_scale<<<n, kThreads, 0, st>>>(t, factor);
+        end = start;
     }
     return rec_launched(fn);
 }

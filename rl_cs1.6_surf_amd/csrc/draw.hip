@@ -494,14 +494,15 @@ struct Block {
         const int b = (int)((-z - from) * (kBins / (to - from)));
         return b < kBins ? b : kBins - 1;
     }
-    // Fills the bins with a range; with top-p, masses too.
-    __device__ __forceinline__ void fill(int range) {
+    // Fills the bins with a range: counts, for a threshold by count, and with
+    // top-p masses.
+    __device__ __forceinline__ void fill(int range, bool counts) {
         clear();
         candidates([&](float x) {
             const float zx = z(x);
             const int b = bin_of(zx, range);
             if (b >= 0) {
-                atomicAdd(&sh.count[b], 1u);
+                if (counts) atomicAdd(&sh.count[b], 1u);
                 if (s.cut) atomicAdd(&sh.mass[b], weight(expf(zx)));
             }
         });
@@ -544,22 +545,24 @@ struct Block {
         __syncthreads();
         return sh.bin < kBins;
     }
-    // Keys of one bin, between lo and hi, into the list if they fit, and their
-    // lowest and highest.
-    __device__ __forceinline__ void collect(int range, int bin, uint32_t lo, uint32_t hi, uint32_t members) {
+    // Keys of one bin, between lo and hi, into the list as far as they fit, and
+    // their lowest and highest; how many there are.
+    __device__ __forceinline__ uint32_t collect(int range, int bin, uint32_t lo, uint32_t hi) {
         clear_list();
         have = -1;
         candidates([&](float x) {
             if (bin_of(z(x), range) == bin) {
                 const uint32_t k = key_of(x);
                 if (k >= lo && k <= hi) {
-                    if (members <= kList) sh.list[atomicAdd(&sh.fill, 1u)] = k;
+                    const uint32_t at = atomicAdd(&sh.fill, 1u);
+                    if (at < kList) sh.list[at] = k;
                     atomicMin(&sh.lo, k);
                     atomicMax(&sh.hi, k);
                 }
             }
         });
         __syncthreads();
+        return sh.fill;
     }
     // The threshold at which the running count or mass, from the top, reaches
     // `bound`; `kept`: the mass up to there (with top-p). False where it lies
@@ -567,18 +570,17 @@ struct Block {
     __device__ __forceinline__ bool threshold(bool by_mass, u64 bound, Cut* cut, u64* kept) {
         u64 above_c = 0, above_m = 0;
         int range = have;
-        if (range < 0) fill(range = by_mass ? kRangeAll : kRangeNear);
+        if (range < 0) fill(range = by_mass || listed ? kRangeAll : kRangeNear, !by_mass);
         if (!find(by_mass, bound)) {
             if (range != kRangeNear) return false;
             totals(&above_c, &above_m);
-            fill(range = kRangeFar);
+            fill(range = kRangeFar, !by_mass);
             if (!find(by_mass, bound - (by_mass ? above_m : above_c))) return false;
         }
         const int bin = (int)sh.bin;
-        uint32_t members = sh.count[bin];
         above_c += sh.above_count;
         above_m += sh.above_mass;
-        collect(range, bin, 0, 0xffffffffu, members);
+        uint32_t members = collect(range, bin, 0, 0xffffffffu);
         uint32_t lo = sh.lo, hi = sh.hi;
         while (members > kList && lo != hi) {
             int shift = 0;
@@ -588,18 +590,17 @@ struct Block {
                 if (bin_of(z(x), range) == bin) {
                     const uint32_t k = key_of(x);
                     if (k >= lo && k <= hi) {
-                        atomicAdd(&sh.count[(hi - k) >> shift], 1u);
+                        if (!by_mass) atomicAdd(&sh.count[(hi - k) >> shift], 1u);
                         if (s.cut) atomicAdd(&sh.mass[(hi - k) >> shift], w(x));
                     }
                 }
             });
             find(by_mass, bound - (by_mass ? above_m : above_c));
             const uint32_t q = sh.bin;   // its keys: hi - k from q << shift on, 1 << shift of them
-            members = sh.count[q];
             above_c += sh.above_count;
             above_m += sh.above_mass;
             const uint32_t top = hi - (q << shift), width = (1u << shift) - 1;
-            collect(range, bin, top - lo < width ? lo : top - width, top, members);
+            members = collect(range, bin, top - lo < width ? lo : top - width, top);
             lo = sh.lo;
             hi = sh.hi;
         }
@@ -637,23 +638,23 @@ struct Block {
         return true;
     }
     // A logit that at least `want` candidates reach, going by the threads' group
-    // maxima; false if none is found within kNear.
+    // maxima; false if none is found within kFar.
     __device__ __forceinline__ bool bound_of(const float (&group)[kGroups], int want, float* bound) {
         clear();
         have = -1;
 #pragma unroll
         for (int q = 0; q < kGroups; ++q) {
-            const int b = bin_of(z(group[q]), kRangeNear);
+            const int b = bin_of(z(group[q]), kRangeAll);
             if (b >= 0) atomicAdd(&sh.count[b], 1u);
         }
         if (!find(false, (u64)want)) return false;
-        *bound = logit_below(sh.bin, kNear);
+        *bound = logit_below(sh.bin);
         return true;
     }
-    // A logit no higher than those of a bin of a range from 0 `to`. (A list may
-    // hold more than it has to, so what is rounded off goes to be safe.)
-    __device__ __forceinline__ float logit_below(uint32_t bin, float to) const {
-        return m - (float)(bin + 2) * (to / kBins) / inv_t;
+    // A logit no higher than those of a bin of kRangeAll. (A list may hold more
+    // than it has to, so what is rounded off goes to be safe.)
+    __device__ __forceinline__ float logit_below(uint32_t bin) const {
+        return m - (float)(bin + 2) * (kFar / kBins) / inv_t;
     }
     // Lists the candidates that reach `bound`; false (and nothing listed) where
     // they do not fit or are fewer than `want`.
@@ -766,18 +767,27 @@ __global__ __launch_bounds__(THREADS) void draw_large(DrawArgs a) {
             b.have = -1;
             if (!of_k) {   // a share of all there is
                 b.listed = 0;
-                b.fill(kRangeAll);
+                b.fill(kRangeAll, false);
                 u64 count;
                 b.totals(&count, &kept);
             }
             u64 share_of = share(s.p24, kept, true);
             if (share_of == 0) share_of = 1;
-            if (!of_k && b.find(true, share_of) && sh.above_count + sh.count[sh.bin] <= B::kCandidates &&
-                b.make_list(b.logit_below(sh.bin, kFar), 1)) {
-                // (rounding at logits of a million and more could leave some out)
-                u64 mass = 0;
-                b.candidates([&](float x) { mass += b.w(x); });
-                if (b.sum(mass) < share_of) b.listed = 0;
+            if (!of_k && b.find(true, share_of)) {
+                // a list, if it has the promise to fit: a little over half the
+                // groups reach that far
+                bound = b.logit_below(sh.bin);
+                u64 groups = 0;
+#pragma unroll
+                for (int q = 0; q < kGroups; ++q) groups += group[q] >= bound;
+                if (b.sum(groups) <= THREADS * kGroups * 9 / 16) {
+                    if (b.make_list(bound, 1)) {
+                        // (rounding at logits of a million and more could leave some out)
+                        u64 mass = 0;
+                        b.candidates([&](float x) { mass += b.w(x); });
+                        if (b.sum(mass) < share_of) b.listed = 0;
+                    }
+                }
             }
             b.threshold(true, share_of, &cut, &kept);
         } else if (!of_k && s.min_p > 0.0f) {
@@ -793,21 +803,39 @@ __global__ __launch_bounds__(THREADS) void draw_large(DrawArgs a) {
     sh.ties[threadIdx.x] = 0;
     __syncthreads();
     if (b.listed) {
-        // all that is kept is in the list, unless only some of the ties are (the
-        // first ones, which the row knows): the kept mass of each stretch of
-        // indices, the stretch that holds the answer, and in it the candidates
+        // all that is kept is in the list. Of the ties at the threshold the first
+        // ones by index are: those after them leave it (with too many ties to
+        // rank the row is gone through instead)
+        u64 ties = 0;
+        for (int i = threadIdx.x; i < b.listed; i += THREADS) ties += sh.key_of[i] == cut.key;
+        ties = b.sum(ties);
+        if (ties > cut.take && ties <= kList) {
+            b.clear_list();
+            for (int i = threadIdx.x; i < b.listed; i += THREADS)
+                if (sh.key_of[i] == cut.key) sh.list[atomicAdd(&sh.fill, 1u)] = sh.index_of[i];
+            __syncthreads();
+            for (int i = threadIdx.x; i < b.listed; i += THREADS)
+                if (sh.key_of[i] == cut.key) {
+                    u64 rank = 0;
+                    for (int q = 0; q < (int)ties; ++q) rank += sh.list[q] < sh.index_of[i];
+                    if (rank >= cut.take) sh.key_of[i] = 0;   // below any threshold
+                }
+            ties = cut.take;
+            __syncthreads();
+        }
+        // the kept mass of each stretch of indices, the stretch that holds the
+        // answer, and in it the candidates
         int width = 0;   // bits of a stretch
         while ((a.vocab - 1) >> width >= THREADS) ++width;
-        u64 ties = 0;
-        for (int i = threadIdx.x; i < b.listed; i += THREADS) {
-            const uint32_t k = sh.key_of[i];
-            ties += k == cut.key;
-            if (k >= cut.key) {
-                const float e = expf(b.z(of_key(k)));
-                if (e >= s.min_p) atomicAdd(&sh.turn[sh.index_of[i] >> width], weight(e));
+        if (ties <= cut.take) {
+            for (int i = threadIdx.x; i < b.listed; i += THREADS) {
+                const uint32_t k = sh.key_of[i];
+                if (k >= cut.key && k != 0) {
+                    const float e = expf(b.z(of_key(k)));
+                    if (e >= s.min_p) atomicAdd(&sh.turn[sh.index_of[i] >> width], weight(e));
+                }
             }
-        }
-        if (b.sum(ties) <= cut.take) {   // (its barriers end the sums above)
+            __syncthreads();
             const u64 mine = sh.turn[threadIdx.x];
             u64 total;
             const u64 before = b.scan(mine, &total);
@@ -822,7 +850,7 @@ __global__ __launch_bounds__(THREADS) void draw_large(DrawArgs a) {
             u64* kept_w = sh.mass;   // of the stretch's candidates, at most 256
             for (int i = threadIdx.x; i < b.listed; i += THREADS) {
                 const uint32_t k = sh.key_of[i], x = sh.index_of[i];
-                if (x >> width != at || k < cut.key) continue;
+                if (x >> width != at || k < cut.key || k == 0) continue;
                 const float e = expf(b.z(of_key(k)));
                 if (!(e >= s.min_p)) continue;
                 const uint32_t q = atomicAdd(&sh.fill, 1u);

@@ -415,12 +415,14 @@ def draw_actions(logits, uniform, *, temperature=1.0, top_k=0, top_p=1.0, min_p=
 
 
 # --------------------------------------------------------------------- clip --
-def _gradient(name, t):
+def _refuse_gradient(t, name):
     if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype not in _CODES:
         raise ValueError(f"{name} must be float32, float16 or bfloat16 tensors on a ROCm GPU; there is no CPU path")
-    if not t.is_contiguous() and not torch._prims_common.is_non_overlapping_and_dense(t):
-        raise ValueError(f"{name} must hold each of their elements once, without gaps")
-    return t
+    raise ValueError(f"{name} must be on one device and hold each of their elements once, without gaps")
+
+
+def _is_dense(t) -> bool:
+    return t.is_contiguous() or torch._prims_common.is_non_overlapping_and_dense(t)
 
 
 _table_packers: dict = {}    # struct.pack of tables of so many tensors
@@ -437,22 +439,26 @@ def clip_grad_norm(grads, max_norm: float, *, out=None, eps: float = 1e-6):
     """The 2-norm over all elements of ``grads`` (tensors of any of the three types, mixed), a float32 scalar on the
     device, and each of them times min(1, max_norm / (norm + eps)): in place, or into the tensors of ``out``
     (``grads`` then stay as they are). A norm that is infinite or NaN goes into the gradients as such."""
-    grads = [_gradient("grads", g) for g in ([grads] if isinstance(grads, torch.Tensor) else grads) if g is not None]
+    grads = [g for g in ((grads,) if isinstance(grads, torch.Tensor) else grads) if g is not None]
     if not grads:
         raise ValueError("no gradients")
-    first = grads[0]
-    index = first.get_device()
-    into = grads if out is None else [_gradient("out", o) for o in ([out] if isinstance(out, torch.Tensor) else out)]
+    into = grads if out is None else (out,) if isinstance(out, torch.Tensor) else list(out)
     if len(into) != len(grads):
         raise ValueError(f"{len(grads)} gradients, {len(into)} places for them")
+    first = grads[0]
+    index = first.get_device() if isinstance(first, torch.Tensor) else -1
     flat = []
     for g, o in zip(grads, into):
-        if g.get_device() != index:
-            raise ValueError(f"gradients on {first.device} and {g.device}")
-        if o is not g and (o.dtype is not g.dtype or o.shape != g.shape or o.stride() != g.stride()
-                           or o.get_device() != index):
-            raise ValueError("out must match the gradients in type, shape, strides and device")
-        flat += (g.data_ptr(), o.data_ptr(), g.numel(), _CODES[g.dtype])
+        dtype = g.dtype if isinstance(g, torch.Tensor) else None
+        code = _CODES.get(dtype)
+        if code is None or g.get_device() != index or index < 0 or not _is_dense(g):
+            _refuse_gradient(g, "grads")
+        if o is not g:
+            if not isinstance(o, torch.Tensor) or o.dtype is not dtype or o.shape != g.shape \
+                    or o.get_device() != index or (o.stride() != g.stride() and not (o.is_contiguous()
+                                                                                     and g.is_contiguous())):
+                raise ValueError("out must match the gradients in type, shape, strides and device")
+        flat += (g.data_ptr(), o.data_ptr(), g.numel(), code)
     table = _table(len(grads))(*flat)
     norm = torch.empty((), dtype=torch.float32, device=first.device)
     ws = _workspace(_sdfr.packed("sdfr_clip_workspace_bytes")(table, len(grads)), first.device)
