@@ -12,7 +12,9 @@ an import hook, before any of those imports, that serves
   the grid contract, the GPU SDF bake);
 * ``surfgym.goalfield`` -> this package's goalfield.py (GPU goal-field bake
   and sampler, EuclidField), unless ``goalfield=False``;
-* ``surfgym._sdfr``     -> the ctypes binding both of them use;
+* ``surfgym.recurrent`` -> this package's recurrent.py (the operators of a policy
+  with a memory; the reference has no module of that name);
+* ``surfgym._sdfr``     -> the ctypes binding they all use;
 
 as members of the reference's own package, so everything else (the core,
 rewards, zones, surfmask, ...) stays the reference's and imports these names
@@ -36,7 +38,7 @@ from pathlib import Path
 
 IMPL = Path(__file__).resolve().parent / "surfgym"
 PACKAGE = "surfgym"
-_SERVED = ("vision", "goalfield", "_sdfr")
+_SERVED = ("vision", "goalfield", "recurrent", "_sdfr")
 
 __all__ = ["install", "uninstall", "installed"]
 
@@ -75,7 +77,7 @@ def install(goalfield: bool = True):
     """Make later imports of ``surfgym.vision`` (and ``surfgym.goalfield``)
     load this package's modules. Raises if the reference's version of one of
     them is already imported: the hook has to run before the first import."""
-    leaves = ["vision", "_sdfr"] + (["goalfield"] if goalfield else [])
+    leaves = [leaf for leaf in _SERVED if goalfield or leaf != "goalfield"]
     for leaf in leaves:
         m = sys.modules.get(f"{PACKAGE}.{leaf}")
         if m is not None and not _is_ours(m):
