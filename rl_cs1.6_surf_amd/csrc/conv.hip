@@ -15,9 +15,13 @@
 //
 // A thread takes four channels of one sequence and walks a run of steps with
 // the window in registers, so inputs are read once but for the run's first
-// width-1 rows; the next four steps' rows are on their way meanwhile. Where a
+// width-1 rows; the next steps' rows are on their way meanwhile. Where a
 // sequence begins the window is emptied, so a step only looks for a beginning
-// at itself.
+// at itself. Memory bounds it: 256 x 128 x 512 bf16 forwards 15 us without
+// beginnings (67 MB at 4.5 TB/s) and 21 with them (the waves that meet one are
+// the last to end), backwards 56 and 62 us (63% of the cycles wait
+// for loads, with 2 waves a SIMD by its registers; 120 steps instead of 128,
+// whose runs do not start a power of two apart, take 38).
 
 #include "recurrent.h"
 
@@ -325,7 +329,8 @@ __global__ __launch_bounds__(kThreads) void conv_forward(ConvArgs a) {
 
 // ---- a single step -------------------------------------------------------------
 // What it moves is the window; the weights, as many bytes again, are read once
-// for kRows sequences.
+// for kRows sequences. 2048 x 512 bf16: 8 us for 17 MB, a launch's time as much
+// as the memory's.
 constexpr int kRows = 4;
 
 template <typename T, int W>

@@ -225,7 +225,8 @@ __device__ inline uint32_t whole_key(uint32_t k) {
 
 // ---- small vocabularies: a wave a row ------------------------------------------
 // All of a row's weights are in registers; the thresholds are searched bit by
-// bit, counts by ballots.
+// bit, counts by ballots. 2048 rows of 243: 5.0 us, a launch and a row's chain
+// of operations; with top-k 8.8, with top-p 19 (32 sums over the wave).
 template <typename T, int E>   // E: candidates a lane
 __global__ __launch_bounds__(256) void draw_small(DrawArgs a) {
     constexpr int V = Row<T>::V, TURNS = E / V;
@@ -360,6 +361,13 @@ __global__ __launch_bounds__(256) void draw_small(DrawArgs a) {
 // of them lie, going by the largest of each of a few thousand groups, which the
 // pass that finds the largest of all keeps; with top-p alone those down to the
 // bin of the threshold; with min-p alone those above that.
+//
+// 256 rows of 131072 bf16, a row a CU: the largest alone 16 us (67 MB at 4.2
+// TB/s), top-k 50 39, with top-p after it 46: the row once more through the
+// caches, then barriers. Without top-k every weight counts, and some 35 vector
+// instructions a logit bound it: no filter 58 us, top-p 106 (spread logits,
+// where a third of the row is kept and nothing fits a list: 151). One row of
+// 50001 with top-k and top-p: 29 us, a CU's loads and the barriers.
 //
 // A top-p threshold after a top-k one needs no list of what top-k left: its
 // bound is a share of that mass, which is reached at or above the top-k key,

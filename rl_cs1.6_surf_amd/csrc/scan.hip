@@ -24,7 +24,15 @@
 // Few sequences: the walk is cut into chunks that run side by side. A first
 // pass walks each chunk from zero and keeps only its end and the product of
 // its decays, scan_join strings them together, and the real pass starts every
-// chunk from its own state.
+// chunk from its own state. (1 x 8192 x 1024 bf16: 40 us for the ends, 11 to
+// join them, 47 for the walk; its 16 waves alone would take 8192 steps one
+// after another.)
+//
+// What bounds it is vector issue, not bytes: a state costs a step two
+// products, an exponential (two slots) and two fused products, 24 cycles of a
+// SIMD for 64 channels, and a channel some 50 slots more. 256 x 128 x 512 bf16
+// with 16 states: forwards 113 us (73% of the cycles issue vector
+// instructions; 298 MB take 57 us), backwards 290 (91%).
 
 #include "recurrent.h"
 
@@ -346,9 +354,11 @@ __global__ __launch_bounds__(256) void scan_join(float* ends, const float* prods
 }
 
 // ---- backward --------------------------------------------------------------
+// dB and dC are sums over channels, which is over lanes: 2 N values a step.
 // Sums over the 64 lanes of 64 values a lane, folded in pairs: at every level
 // a lane keeps one of two values and takes its partner's share of it, so a
-// value costs about two instructions instead of six. Level j pairs values
+// value costs about two instructions instead of six (a seventh of the walk
+// back). Level j pairs values
 // whose index differs in bit j and lanes that differ in bit 5 - j.
 template <int LEVEL>
 __device__ inline float fold(float a, float b) {
@@ -501,7 +511,7 @@ __global__ __launch_bounds__(64 * kWaves) void scan_backward_ends(ScanArgs a, Gr
 // The walk back goes by tiles of half the marks' distance, whose kept states
 // (64 registers) it works out forwards first: the lower tile of a pair from the
 // mark, the upper one by going over the lower one too (an eighth more work; with
-// whole tiles' 128 registers the kernel spills and takes six times as long).
+// whole tiles' 128 registers the kernel spilled, 1125 us where this took 332).
 //
 // As in scan_forward there are two copies of a tile, without branches and with.
 // Lanes past the last channel repeat it, and write what it writes, but add
@@ -758,7 +768,8 @@ __global__ __launch_bounds__(1024) void column_sums(const float* __restrict__ su
 // ---- a single token ----------------------------------------------------------
 // What bounds it is the state, read and written once: a lane takes four states
 // of a channel (one 16-byte load and store), LANES lanes a channel, and the sum
-// over states is folded over those lanes.
+// over states is folded over those lanes. 2048 x 1024 x 16: 61.6 us, 285 MB at
+// 4.6 TB/s (a large copy reaches 5.2).
 template <typename T, int LANES, bool WIDE>
 __global__ __launch_bounds__(256) void scan_step(ScanArgs a, Rows B, Rows C) {
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
