@@ -986,6 +986,14 @@ SDFR_API int32_t sdfr_draw(const SdfrDraw* s, void* stream) {
     a.logp = s->logp;
     a.rows = s->rows;
     a.vocab = s->vocab;
+    // Which kernel (bf16, no filter / top-k 50 / top-p 0.9 / both, us): a wave a
+    // row up to 1024, what its registers hold: 2048 rows of 1000 8 / 11 / 19 / 28,
+    // by a workgroup 20 / 24 / 33 / 32. Workgroups of 256 threads, several a CU,
+    // up to 16384 (512 rows of 16000 23 / 20 / 41 / 23, 1024 threads 29 / 36 / 61 /
+    // 50; one row of 20000 22 / 18 / 41 / 21 and 17 / 19 / 33 / 26), and up to
+    // 65536, as far as a stretch's candidates fit kList, where there are more rows
+    // than CUs (512 rows of 60000 63 / 37 / 115 / 40 and 68 / 53 / 122 / 66; 256
+    // rows 53 / 33 / 100 / 36 and 33 / 26 / 61 / 32).
     rec_typed(s->dtype, [&](auto v) {
         typedef decltype(v) T;
         const unsigned small = (unsigned)((s->rows + 3) / 4);
@@ -993,7 +1001,7 @@ SDFR_API int32_t sdfr_draw(const SdfrDraw* s, void* stream) {
             draw_small<T, 8><<<small, 256, 0, st>>>(a);
         else if (s->vocab <= 1024)
             draw_small<T, 16><<<small, 256, 0, st>>>(a);
-        else if (s->vocab <= 8192)
+        else if (s->vocab <= (s->rows > 256 ? 65536 : 16384))
             draw_large<T, 256><<<s->rows, 256, 0, st>>>(a);
         else
             draw_large<T, 1024><<<s->rows, 1024, 0, st>>>(a);
