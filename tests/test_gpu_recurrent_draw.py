@@ -290,3 +290,45 @@ def test_clip_refusals(dev):
     from surfgym import _sdfr
     with pytest.raises(_sdfr.SdfrError, match="negative"):
         ops.clip_grad_norm([g], -1.0)
+
+
+@pytest.mark.parametrize("vocab", [9000, 20011, 65536, 70001])
+def test_many_rows_draw_as_few_do(dev, vocab):
+    """More rows than compute units may take another kernel; the answers are the same bits."""
+    x = (torch.randn(300, vocab, generator=_gen(vocab)) * 3).to(torch.bfloat16).to(dev)
+    u = torch.rand(300, generator=_gen(1)).to(dev)
+    for s in (dict(), dict(top_k=50), dict(top_p=0.9), dict(top_k=700, top_p=0.95, min_p=0.01), dict(min_p=0.02)):
+        token, logp = ops.draw_actions(x, u, **s)
+        for at in (0, 100, 200):
+            t, p = ops.draw_actions(x[at:at + 100], u[at:at + 100], **s)
+            assert torch.equal(t, token[at:at + 100]) and torch.equal(p, logp[at:at + 100])
+
+
+@pytest.mark.parametrize("vocab", [3000, 20000, 100000])
+@pytest.mark.parametrize("equal", [100, 250, 300, 1000])
+def test_some_of_many_equal_candidates(dev, vocab, equal):
+    """Thresholds that fall among equal logits, few enough to rank and more."""
+    g = _gen(vocab + equal)
+    x = torch.randn(4, vocab, generator=g)
+    for i in range(4):
+        x[i, torch.randperm(vocab, generator=g)[:equal]] = 6.0
+        x[i, torch.randperm(vocab, generator=g)[:5]] = 7.0
+    for s in (dict(top_k=equal // 2), dict(top_k=equal // 2, top_p=0.6), dict(top_p=0.3), dict(top_k=5 + equal, top_p=0.9)):
+        print("case equal", vocab, equal, s, flush=True)
+        _check(dev, x, s, seed=3)
+
+
+@pytest.mark.parametrize("vocab", [700, 3000, 20011])
+def test_far_apart_and_far_from_zero(dev, vocab):
+    """One logit so far above that the others weigh nothing; logits whose spacing is a sixteenth; tiny and huge
+    temperatures."""
+    g = _gen(vocab)
+    x = torch.randn(4, vocab, generator=g)
+    x[0, vocab // 3] = 100.0
+    x[1, vocab // 3], x[1, vocab // 2] = 100.0, 100.0
+    x[2] = x[2] * 3 + 1e6
+    x[3] = x[3] * 3 - 1e6
+    for s in (dict(top_k=50), dict(top_k=50, top_p=0.9), dict(top_p=0.9), dict(min_p=0.1), dict(temperature=1e-3, top_p=0.9),
+              dict(temperature=1e4, top_p=0.5), dict(temperature=1e4, top_k=20, min_p=0.5)):
+        print("case far", vocab, s, flush=True)
+        _check(dev, x, s, seed=5)
