@@ -7,7 +7,7 @@
 // clip_scale multiplies. Squares and sums are fp64: no square of an fp32 value
 // overflows, and the memory is what bounds it either way.
 //
-// 400 M bf16 elements: 512 us for 2.4 GB, 4.7 TB/s, of which the second read
+// 400 M bf16 elements: 514 us for 2.4 GB, 4.7 TB/s, of which the second read
 // could be saved only by gradients that fit the caches; 2 M fp32 ones: 4.4, 4.1
 // and 5.0 us, launches.
 //
