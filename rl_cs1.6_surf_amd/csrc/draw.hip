@@ -369,6 +369,10 @@ __global__ __launch_bounds__(256) void draw_small(DrawArgs a) {
 // where a third of the row is kept and nothing fits a list: 151). One row of
 // 50001 with top-k and top-p: 29 us, a CU's loads and the barriers.
 //
+// A short list goes through the bins as well: its 256 keys ranked whole, and
+// each adding up those before it, need fewer barriers but as many LDS reads one
+// after another (2048 rows of 8000 bf16: top-k 50 30 -> 35 us, top-p 56 -> 78).
+//
 // A top-p threshold after a top-k one needs no list of what top-k left: its
 // bound is a share of that mass, which is reached at or above the top-k key,
 // and among the ties there no later than the last one taken.
